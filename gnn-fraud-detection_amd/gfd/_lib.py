@@ -17,6 +17,7 @@ LIB_PATH = os.environ.get("GFD_LIB_PATH") or os.path.join(
     os.path.dirname(os.path.abspath(__file__)), "libgfd.so")
 
 c_i32, c_i64, c_u64, c_f32, c_sz = ct.c_int32, ct.c_int64, ct.c_uint64, ct.c_float, ct.c_size_t
+c_f64 = ct.c_double
 P = ct.c_void_p
 
 
@@ -36,7 +37,7 @@ class GfdPlan(ct.Structure):
 
 
 # element types of x (GFD_DTYPE_*)
-DTYPE_F32, DTYPE_BF16 = 0, 1
+DTYPE_F32, DTYPE_BF16, DTYPE_F16 = 0, 1, 2
 
 
 def x_dtype_code(t) -> int:
@@ -136,6 +137,18 @@ SIGNATURES = {
                                  c_i64, P, P, P, ct.c_int, ct.c_int, c_f32, c_f32, c_u64, P, P, P,
                                  P, P, P, P, P, P, ct.c_int, P, c_sz, P]),
     "gfd_x_colmax": (c_i32, [P, ct.c_int, c_i64, ct.c_int, c_i64, P, P]),
+    "gfd_group_norm_workspace_size": (c_sz, [c_i64, c_i64, ct.c_int, ct.c_int, ct.c_int, ct.c_int]),
+    "gfd_group_norm_fwd": (c_i32, [P, ct.c_int, c_i64, c_i64, P, ct.c_int, ct.c_int, c_i64, c_i64,
+                                   P, P, ct.c_int, c_f64, ct.c_int, P, P, P, c_sz, P]),
+    "gfd_group_norm_bwd": (c_i32, [P, ct.c_int, c_i64, c_i64, P, ct.c_int, ct.c_int, c_i64, c_i64,
+                                   P, P, ct.c_int, ct.c_int, P, P, P, P, P, P, c_sz, P]),
+    "gfd_class_logp_workspace_size": (c_sz, [c_i64, c_i64, ct.c_int]),
+    "gfd_class_logp_fwd": (c_i32, [P, ct.c_int, c_i64, c_i64, c_i64, P, c_i64, ct.c_int, P, P, P,
+                                   P, P, P, c_sz, P]),
+    "gfd_class_logp_bwd": (c_i32, [P, ct.c_int, c_i64, c_i64, c_i64, P, c_i64, ct.c_int, P, P, P,
+                                   P, P, P, P, P]),
+    "gfd_adam_step": (c_i32, [P, c_i64, ct.c_int, ct.c_int, P, P, P, P, P, c_f64, P, c_f64, c_f64,
+                              c_f64, c_f64, ct.c_int, ct.c_uint32, P, P]),
 }
 
 STATUS = {0: "ok", 1: "invalid argument", 2: "edge index out of range", 3: "workspace too small",
@@ -185,6 +198,15 @@ def call(name: str, *args):
     if st != 0:
         raise GfdError(name, st)
     return st
+
+
+def call_on(device, name: str, *args):
+    """``call`` with ``device`` as the current HIP device (a launch goes to the current one)."""
+    import torch
+    if device.index is None or device.index == torch.cuda.current_device():
+        return call(name, *args)
+    with torch.cuda.device(device):
+        return call(name, *args)
 
 
 def ptr(t) -> int | None:

@@ -46,8 +46,10 @@ BASE_FLAGS = ["-O3", "-std=c++17", "-fPIC", f"--offload-arch={ARCH}", "-munsafe-
 # the variants build() always produces next to the product library:
 #   checked -- the bounds-checked diagnostic build (gfd_check.h)
 SHIPPED_VARIANTS = {"checked": ["-DGFD_CHECKED"]}
-# Per-source flags: {"file.hip": [flags]}
-SOURCE_FLAGS = {}
+# Per-source flags: {"file.hip": [flags]}.  The row-wise training operators carry NaN and
+# infinity through as the formulas do
+SOURCE_FLAGS = {name: ["-fhonor-nans"]
+                for name in ("gfd_adam.hip", "gfd_class_logp.hip", "gfd_group_norm.hip")}
 
 
 def lib_path(variant: str = "") -> str:
@@ -113,6 +115,7 @@ def source_id(flags=None) -> str:
         with open(p, "rb") as f:
             h.update(f.read())
     h.update(" ".join(flags if flags is not None else FLAGS).encode())
+    h.update(repr(sorted(SOURCE_FLAGS.items())).encode())
     h.update(ARCH.encode())
     return h.hexdigest()
 

@@ -762,6 +762,9 @@ def model_forward_sharded(model, x: torch.Tensor, graph, spec: ShardSpec, group=
     destinations, or of all N nodes (gather_output).  Inference only."""
     if model.training or torch.is_grad_enabled():
         raise RuntimeError("model_forward_sharded is inference-only: model.eval() and no_grad")
+    if getattr(model, "group_norms", None) is not None:
+        raise NotImplementedError("model_forward_sharded: norm='group' models (the layer epilogue "
+                                  "folds a BatchNorm); use gat_forward_sharded_train under no_grad")
     if exchange not in ("halo", "allgather"):
         raise ValueError(f"exchange must be 'halo' or 'allgather', got {exchange!r}")
     h = x
@@ -1088,7 +1091,10 @@ def gat_forward_sharded_train(model, x: torch.Tensor, local: LocalGraph, plan: H
     for li, conv in enumerate(model.gat_layers):
         x_local = local.rows(x) if li == 0 else halo_rows(h_own, plan, lo, group)
         y = conv_fn(conv, x_local, local, model.training)
-        if model.batch_norms is not None:
+        if getattr(model, "group_norms", None) is not None:
+            # a node's own statistics: nothing to exchange (the relu is the norm's)
+            y = model.group_norms[li](y)
+        elif model.batch_norms is not None:
             bn = model.batch_norms[li]
             # eval: the running statistics, identical on every rank
             y = sharded_batch_norm(y, bn, n_total, group) if model.training else bn(y)

@@ -18,14 +18,22 @@
   passes over y each way instead of ATen's BN / relu / dropout / add chain
   and its saved intermediates; only y and two [64] vectors are kept).
 
+* ``group_norm`` -- group norm with an activation over node rows (dense or
+  ragged segments), forward and backward (``gfd_group_norm_fwd`` / ``_bwd``):
+  statistics that stay inside a node, a snapshot or a sampled subgraph.
+* ``class_log_probs`` -- log probabilities of given classes with entropy and
+  top alternatives from a classification head's logits, forward and backward
+  (``gfd_class_logp_fwd`` / ``_bwd``).
+
 ``gat_layer`` and ``gru_head`` are inference-only: they refuse tensors that
 require grad (gfd.models takes ``GATConv`` + ``train_body`` then).
 """
 from __future__ import annotations
 
-from typing import Optional, Tuple
+from typing import NamedTuple, Optional, Tuple
 
 import torch
+from torch.autograd.function import once_differentiable
 
 from . import _lib
 from .graph import CSRGraph, _ws, get_graph
@@ -367,3 +375,207 @@ def train_body(y: torch.Tensor, bn: torch.nn.BatchNorm1d, h: Optional[torch.Tens
         res = h if (h.dtype == torch.float32 and h.is_contiguous()) else h.float().contiguous()
     seed = int(torch.randint(0, 2 ** 62, (1,)).item()) if p > 0 else 0
     return _BNReluDropout.apply(y, res, bn.weight, bn.bias, bn, relu, p, seed)
+
+
+# ---------------------------------------------------------------------------
+# row-wise training operators
+# ---------------------------------------------------------------------------
+
+_ROW_DTYPES = {torch.float32: _lib.DTYPE_F32, torch.bfloat16: _lib.DTYPE_BF16,
+               torch.float16: _lib.DTYPE_F16}
+ACTIVATIONS = {"none": 0, "relu": 1, "silu": 2, "gelu": 3}
+
+
+def _check_rows(what: str, name: str, t: torch.Tensor) -> None:
+    if not t.is_cuda:
+        raise RuntimeError(f"gfd {what}: {name} must be on a HIP device (got {t.device})")
+    if t.dtype not in _ROW_DTYPES:
+        raise TypeError(f"gfd {what}: {name} must be float32, bfloat16 or float16 (got {t.dtype})")
+
+
+class _GroupNorm(torch.autograd.Function):
+    """act(group_norm(x)) over gfd_group_norm_fwd / _bwd; x [B, L, C] (dense) or
+    [N, C] with ptr (ragged).  x and the fp64 statistics are kept."""
+
+    @staticmethod
+    def forward(ctx, x, weight, bias, ptr, groups, eps, act, grad_mode):
+        dev, ragged = x.device, ptr is not None
+        C = x.size(-1)
+        segments, length = (ptr.numel() - 1, x.size(0)) if ragged else (x.size(0), x.size(1))
+        keep = grad_mode and any(ctx.needs_input_grad[:3])
+        y = torch.empty(x.shape, dtype=x.dtype, device=dev)
+        stats = (torch.empty((segments, groups, 2), dtype=torch.float64, device=dev) if keep
+                 else None)
+        ctx.geom = (_ROW_DTYPES[x.dtype], segments, length, _lib.ptr(ptr), C, groups,
+                    x.stride(-2), 0 if ragged else x.stride(0))
+        w_dtype = _ROW_DTYPES[weight.dtype if weight is not None else
+                              bias.dtype if bias is not None else x.dtype]
+        lib = _lib.load()
+        nbytes = lib.gfd_group_norm_workspace_size(segments, length, int(ragged), C, groups, 0)
+        ws = _ws(nbytes, dev) if nbytes else None
+        _lib.call_on(dev, "gfd_group_norm_fwd", x.data_ptr(), *ctx.geom, _lib.ptr(weight),
+                     _lib.ptr(bias), w_dtype, eps, act, y.data_ptr(), _lib.ptr(stats),
+                     _lib.ptr(ws), nbytes, _lib.stream_handle(dev))
+        if keep:
+            ctx.save_for_backward(x, weight, bias, ptr, stats)
+            ctx.act, ctx.w_dtype = act, w_dtype
+        return y
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, grad):
+        x, weight, bias, ptr, stats = ctx.saved_tensors
+        dev = x.device
+        grad = grad.contiguous()
+        gx = torch.empty(x.shape, dtype=x.dtype, device=dev)
+        gw = torch.empty_like(weight) if weight is not None and ctx.needs_input_grad[1] else None
+        gb = torch.empty_like(bias) if bias is not None and ctx.needs_input_grad[2] else None
+        lib = _lib.load()
+        _, segments, length, _, C, groups, _, _ = ctx.geom
+        nbytes = lib.gfd_group_norm_workspace_size(segments, length, int(ptr is not None), C,
+                                                   groups, 1)
+        ws = _ws(nbytes, dev)
+        _lib.call_on(dev, "gfd_group_norm_bwd", x.data_ptr(), *ctx.geom, _lib.ptr(weight),
+                     _lib.ptr(bias), ctx.w_dtype, ctx.act, stats.data_ptr(), grad.data_ptr(),
+                     gx.data_ptr(), _lib.ptr(gw), _lib.ptr(gb), ws.data_ptr(), ws.numel(),
+                     _lib.stream_handle(dev))
+        return gx, gw, gb, None, None, None, None, None
+
+
+def group_norm(x: torch.Tensor, num_groups: int, weight: Optional[torch.Tensor] = None,
+               bias: Optional[torch.Tensor] = None, eps: float = 1e-5, act: str = "none",
+               ptr: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """``act(group_norm(x) * weight + bias)``, channels last, differentiable.
+
+    x [N, C]: every row has its own statistics over the channels of a group;
+    x [B, ..., C]: over all positions of a sample and the channels of a group;
+    x [N, C] with ``ptr`` (int64 [segments + 1] on the device, non-decreasing, as
+    a ragged batch of graphs has): over the rows ptr[s] .. ptr[s + 1] of a
+    segment, which may be empty.  Rows outside of every segment get 0 and no
+    gradient.  x in float32, bfloat16 or float16, C <= 2048; weight / bias [C]
+    in float32 or x's type; ``act`` none, relu, silu or gelu (erf).  The output
+    is contiguous."""
+    _check_rows("group_norm", "x", x)
+    if act not in ACTIVATIONS:
+        raise ValueError(f"gfd group_norm: act must be one of {sorted(ACTIVATIONS)} (got {act!r})")
+    if x.dim() < 2 or (ptr is not None and x.dim() != 2):
+        raise ValueError(f"gfd group_norm: x must be [N, C] or [B, ..., C], with ptr [N, C] (got "
+                         f"{tuple(x.shape)})")
+    C = x.size(-1)
+    if not 1 <= C <= 2048:
+        raise NotImplementedError(f"gfd group_norm: 1 to 2048 channels (got {C})")
+    if num_groups < 1 or C % num_groups:
+        raise ValueError(f"gfd group_norm: {C} channels are not a multiple of {num_groups} groups")
+    if not eps >= 0:
+        raise ValueError(f"gfd group_norm: eps must be >= 0 (got {eps})")
+    for name, t in (("weight", weight), ("bias", bias)):
+        if t is None:
+            continue
+        if t.device != x.device:
+            raise RuntimeError(f"gfd group_norm: {name} is on {t.device}, expected {x.device}")
+        if t.shape != (C,):
+            raise ValueError(f"gfd group_norm: {name} must be [{C}] (got {tuple(t.shape)})")
+        if t.dtype not in (torch.float32, x.dtype) or (weight is not None and t.dtype != weight.dtype):
+            raise TypeError(f"gfd group_norm: weight and bias must both be float32 or {x.dtype} "
+                            f"(got {name} {t.dtype})")
+    if ptr is not None:
+        if ptr.device != x.device or ptr.dtype != torch.int64 or ptr.dim() != 1 or ptr.numel() < 1:
+            raise ValueError("gfd group_norm: ptr must be int64 [segments + 1] on x's device")
+        ptr = ptr.contiguous()
+    shape = x.shape
+    if ptr is None:
+        x = x.unsqueeze(1) if x.dim() == 2 else x.flatten(1, -2)
+    if C > 1 and x.stride(-1) != 1:
+        x = x.contiguous()
+    weight = weight.contiguous() if weight is not None else None
+    bias = bias.contiguous() if bias is not None else None
+    return _GroupNorm.apply(x, weight, bias, ptr, int(num_groups), float(eps), ACTIVATIONS[act],
+                            torch.is_grad_enabled()).view(shape)
+
+
+class ClassLogProbs(NamedTuple):
+    """What ``class_log_probs`` returns; all float32 but the classes (int64)."""
+    log_prob: Optional[torch.Tensor]     # [...] of the given classes; None without a target
+    entropy: torch.Tensor                # [...] natural log
+    top_log_probs: torch.Tensor          # [..., top]
+    top_classes: torch.Tensor            # [..., top]
+
+
+class _ClassLogProbs(torch.autograd.Function):
+    """Over gfd_class_logp_fwd / _bwd: the logits, two statistics and the entropy
+    of a row are kept."""
+
+    @staticmethod
+    def forward(ctx, logits, target, top, ignore_index):
+        dev = logits.device
+        rows, classes = logits.shape
+        f32 = dict(dtype=torch.float32, device=dev)
+        logp = torch.empty(rows, **f32) if target is not None else None
+        entropy = torch.empty(rows, **f32)
+        top_logp = torch.empty((rows, top), **f32)
+        top_class = torch.empty((rows, top), dtype=torch.int64, device=dev)
+        stats = torch.empty((rows, 2), **f32)
+        nbytes = _lib.load().gfd_class_logp_workspace_size(rows, classes, top)
+        ws = _ws(nbytes, dev) if nbytes else None
+        ctx.geom = (_ROW_DTYPES[logits.dtype], rows, classes, logits.stride(0))
+        _lib.call_on(dev, "gfd_class_logp_fwd", logits.data_ptr(), *ctx.geom, _lib.ptr(target),
+                     ignore_index, top, _lib.ptr(logp), entropy.data_ptr(), top_logp.data_ptr(),
+                     top_class.data_ptr(), stats.data_ptr(), _lib.ptr(ws), nbytes,
+                     _lib.stream_handle(dev))
+        ctx.save_for_backward(logits, target, entropy, top_class, stats)
+        ctx.top, ctx.ignore_index = top, ignore_index
+        ctx.mark_non_differentiable(top_class)
+        ctx.set_materialize_grads(False)
+        return logp, entropy, top_logp, top_class
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, g_logp, g_entropy, g_top, _):
+        logits, target, entropy, top_class, stats = ctx.saved_tensors
+        dev = logits.device
+        g_logp, g_entropy, g_top = (g.contiguous() if g is not None else None
+                                    for g in (g_logp, g_entropy, g_top))
+        grad = torch.empty(logits.shape, dtype=logits.dtype, device=dev)
+        _lib.call_on(dev, "gfd_class_logp_bwd", logits.data_ptr(), *ctx.geom, _lib.ptr(target),
+                     ctx.ignore_index, ctx.top, top_class.data_ptr(), stats.data_ptr(),
+                     entropy.data_ptr(), _lib.ptr(g_logp), _lib.ptr(g_entropy), _lib.ptr(g_top),
+                     grad.data_ptr(), _lib.stream_handle(dev))
+        return grad, None, None, None
+
+
+def class_log_probs(logits: torch.Tensor, target: Optional[torch.Tensor] = None, top: int = 0,
+                    ignore_index: int = -1) -> ClassLogProbs:
+    """Log probabilities of the given classes, the entropy and the ``top`` most
+    likely classes with their log probabilities, for logits [..., classes] in
+    float32, bfloat16 or float16 and target int64 [...]; differentiable in the
+    log probabilities and the entropy.
+
+    A target of ``ignore_index`` (the reference's unknown label, -1) has log
+    probability 0 and no gradient; any other one outside of the classes gives NaN.
+    A masked class is a logit of -inf; a row of nothing else has log probability
+    -inf, entropy 0 and no gradient.  Equal logits are listed by the lower class.
+    0 <= top <= min(64, classes)."""
+    _check_rows("class_log_probs", "logits", logits)
+    if logits.dim() < 1 or logits.size(-1) < 1:
+        raise ValueError(f"gfd class_log_probs: logits must be [..., classes] (got {tuple(logits.shape)})")
+    classes, lead = logits.size(-1), logits.shape[:-1]
+    if not 0 <= top <= min(64, classes):
+        raise ValueError(f"gfd class_log_probs: top must be in [0, {min(64, classes)}] (got {top})")
+    if target is not None:
+        if target.device != logits.device:
+            raise RuntimeError(f"gfd class_log_probs: target is on {target.device}, expected "
+                               f"{logits.device}")
+        if target.dtype != torch.int64:
+            raise TypeError(f"gfd class_log_probs: target must be int64 (got {target.dtype})")
+        if target.shape != lead:
+            raise ValueError(f"gfd class_log_probs: target must be {tuple(lead)} (got "
+                             f"{tuple(target.shape)})")
+        target = target.reshape(-1).contiguous()
+    x = logits if logits.dim() == 2 else logits.reshape(-1, classes)
+    if (classes > 1 and x.stride(1) != 1) or x.stride(0) < 0:
+        x = x.contiguous()
+    logp, entropy, top_logp, top_class = _ClassLogProbs.apply(x, target, int(top), int(ignore_index))
+    if logits.dim() == 2:
+        return ClassLogProbs(logp, entropy, top_logp, top_class)
+    return ClassLogProbs(logp.view(lead) if logp is not None else None, entropy.view(lead),
+                         top_logp.view(*lead, top), top_class.view(*lead, top))

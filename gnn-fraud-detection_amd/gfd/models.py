@@ -7,6 +7,10 @@ constructor arguments, same submodule names (so ``results/gat_model.pt`` and
 ``results/tgn_model.pt`` load with ``strict=True``), same outputs.  The only
 difference is the GATConv underneath: ``gfd.nn.GATConv`` (libgfd.so).
 
+Beyond the reference, ``norm="group"`` replaces the BatchNorm by a group norm
+over each node's row (``gfd.nn.GroupNorm``), and ``log_probs`` scores the classes
+of a model with several (``gfd.fused.class_log_probs``).
+
 The per-layer epilogue is the reference's: GATConv -> BatchNorm1d -> ReLU ->
 dropout -> residual when widths match (gat.py:79-91).  In inference (eval mode
 under no_grad) each layer is one fused call (BN folded into the GATConv store
@@ -30,7 +34,7 @@ import torch
 import torch.nn as nn
 import torch.nn.functional as F
 
-from .nn import GATConv
+from .nn import GATConv, GroupNorm
 
 
 class _GATStack(nn.Module):
@@ -38,8 +42,11 @@ class _GATStack(nn.Module):
 
     def __init__(self, in_channels: int, hidden_channels: int, out_channels: int,
                  num_layers: int = 2, dropout: float = 0.2, residual: bool = True,
-                 use_batch_norm: bool = True):
+                 use_batch_norm: bool = True, norm: str = "batch", num_groups: int = 8):
         super().__init__()
+        if norm not in ("batch", "group"):
+            raise ValueError(f"norm must be 'batch' or 'group' (got {norm!r})")
+        use_batch_norm = use_batch_norm and norm == "batch"
         self.in_channels, self.hidden_channels = in_channels, hidden_channels
         self.out_channels, self.num_layers = out_channels, num_layers
         self.dropout, self.residual, self.use_batch_norm = dropout, residual, use_batch_norm
@@ -49,6 +56,10 @@ class _GATStack(nn.Module):
             GATConv(w, hidden_channels, heads=8, concat=False, dropout=dropout) for w in widths)
         self.batch_norms = (nn.ModuleList(nn.BatchNorm1d(hidden_channels) for _ in widths)
                             if use_batch_norm else None)
+        # norm="group": every node's row has its own statistics, so a snapshot, a sampled
+        # batch or a shard is normalised alike in training and inference
+        self.group_norms = (nn.ModuleList(GroupNorm(num_groups, hidden_channels, act="relu")
+                                          for _ in widths) if norm == "group" else None)
 
     def _fused(self) -> bool:
         """Inference (eval mode, no autograd): each layer body runs as one
@@ -59,6 +70,11 @@ class _GATStack(nn.Module):
         """The layer stack; in inference, ``head`` (fused.head_foldable) is
         folded into the last layer's store and its [N, 1] output returned."""
         h = x
+        if self.group_norms is not None:
+            for conv, norm in zip(self.gat_layers, self.group_norms):
+                y = F.dropout(norm(conv(h, edge_index)), p=self.dropout, training=self.training)
+                h = h + y if (self.residual and h.size(-1) == y.size(-1)) else y
+            return h
         if self._fused():
             from . import fused
             last = len(self.gat_layers) - 1
@@ -83,6 +99,19 @@ class _GATStack(nn.Module):
             h = h + y if (self.residual and h.size(-1) == y.size(-1)) else y
         return h
 
+    def log_probs(self, x, edge_index, target: Optional[torch.Tensor] = None, top: int = 0,
+                  ignore_index: int = -1, **kwargs):
+        """Of a model with several classes (out_channels > 1): the log probability of
+        every node's ``target`` class (``ignore_index``, the reference's unknown label:
+        0), the entropy and the ``top`` most likely classes
+        (``gfd.fused.class_log_probs``, differentiable)."""
+        if self.out_channels < 2:
+            raise ValueError("log_probs needs a model with out_channels >= 2 (predict() gives the "
+                             "probability of a single logit)")
+        from .fused import class_log_probs
+        out = self.forward(x, edge_index, **kwargs)
+        return class_log_probs(out[0] if isinstance(out, tuple) else out, target, top, ignore_index)
+
 
 def _head(lin: nn.Linear, h: torch.Tensor) -> torch.Tensor:
     """``lin(h)``.  For the reference's single-logit head (Linear(64, 1),
@@ -101,13 +130,13 @@ class GAT(_GATStack):
 
     def __init__(self, in_channels: int, hidden_channels: int, out_channels: int,
                  num_layers: int = 2, dropout: float = 0.2, residual: bool = True,
-                 use_batch_norm: bool = True):
+                 use_batch_norm: bool = True, norm: str = "batch", num_groups: int = 8):
         super().__init__(in_channels, hidden_channels, out_channels, num_layers, dropout,
-                         residual, use_batch_norm)
+                         residual, use_batch_norm, norm, num_groups)
         self.out = nn.Linear(hidden_channels, out_channels)
 
     def forward(self, x, edge_index, batch: Optional[torch.Tensor] = None) -> torch.Tensor:
-        if self._fused() and x.is_cuda and self.gat_layers:
+        if self._fused() and x.is_cuda and self.gat_layers and self.group_norms is None:
             from .fused import head_foldable
             width = self.gat_layers[-1].in_channels
             if head_foldable(self.out, width, self.gat_layers[-1]):
@@ -126,9 +155,9 @@ class TemporalGNN(_GATStack):
 
     def __init__(self, in_channels: int, hidden_channels: int, out_channels: int,
                  num_layers: int = 2, dropout: float = 0.2, residual: bool = True,
-                 use_batch_norm: bool = True):
+                 use_batch_norm: bool = True, norm: str = "batch", num_groups: int = 8):
         super().__init__(in_channels, hidden_channels, out_channels, num_layers, dropout,
-                         residual, use_batch_norm)
+                         residual, use_batch_norm, norm, num_groups)
         self.gru = nn.GRUCell(hidden_channels, hidden_channels)
         self.out = nn.Linear(hidden_channels, out_channels)
 

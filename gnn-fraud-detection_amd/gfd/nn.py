@@ -230,3 +230,37 @@ class GATConv(nn.Module):
     def extra_repr(self) -> str:
         return (f"{self.in_channels}, {self.out_channels}, heads={self.heads}, concat=False, "
                 f"dropout={self.dropout}")
+
+
+class GroupNorm(nn.Module):
+    """``torch.nn.GroupNorm`` over node rows, channels last, with an activation
+    (``gfd.fused.group_norm``): forward(x [N, C]), (x [B, ..., C]) or (x [N, C],
+    ptr) for a ragged batch of graphs.  Same parameters and state-dict keys."""
+
+    def __init__(self, num_groups: int, num_channels: int, eps: float = 1e-5, affine: bool = True,
+                 act: str = "none"):
+        super().__init__()
+        from .fused import ACTIVATIONS
+        if num_groups < 1 or num_channels % num_groups:
+            raise ValueError("num_channels must be divisible by num_groups")
+        if act not in ACTIVATIONS:
+            raise ValueError(f"act must be one of {sorted(ACTIVATIONS)} (got {act!r})")
+        self.num_groups, self.num_channels, self.eps = num_groups, num_channels, eps
+        self.affine, self.act = affine, act
+        self.weight = nn.Parameter(torch.ones(num_channels)) if affine else None
+        self.bias = nn.Parameter(torch.zeros(num_channels)) if affine else None
+
+    def reset_parameters(self):
+        if self.affine:
+            nn.init.ones_(self.weight)
+            nn.init.zeros_(self.bias)
+
+    def forward(self, x: torch.Tensor, ptr: Optional[torch.Tensor] = None) -> torch.Tensor:
+        from .fused import group_norm
+        if x.size(-1) != self.num_channels:
+            raise ValueError(f"x has {x.size(-1)} channels, the norm expects {self.num_channels}")
+        return group_norm(x, self.num_groups, self.weight, self.bias, self.eps, self.act, ptr)
+
+    def extra_repr(self) -> str:
+        return (f"{self.num_groups}, {self.num_channels}, eps={self.eps}, affine={self.affine}, "
+                f"act={self.act}")

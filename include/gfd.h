@@ -54,6 +54,7 @@ typedef int32_t gfd_status;
 /* Element type of the node features x (``x_dtype`` arguments). */
 #define GFD_DTYPE_F32 0
 #define GFD_DTYPE_BF16 1
+#define GFD_DTYPE_F16 2 /* gfd_group_norm_*, gfd_class_logp_*, gfd_adam_step only */
 
 const char* gfd_status_string(gfd_status status);
 int gfd_abi_version(void);
@@ -579,6 +580,128 @@ gfd_status gfd_bn_relu_bwd(const float* y, const float* grad_out, int64_t N, int
 gfd_status gfd_rows_copy(const float* src, int64_t src_stride, const int32_t* src_rows,
                          float* dst, int64_t dst_stride, const int32_t* dst_rows, int64_t n,
                          int cols, gfd_stream_t stream);
+
+/* ---------------------------------------------------------------------------
+ * Group norm with an activation over node rows, channels last: the sibling of
+ * gfd_bn_relu_fwd whose statistics stay inside a segment of rows (one node,
+ * one snapshot, one sampled subgraph) and a group of channels:
+ *   xhat = (x - mean_sg) / sqrt(var_sg + eps),  y = act(xhat * weight + bias)
+ * with mean and (biased) variance over the rows of segment s and the channels /
+ * groups channels of group g.  Two layouts:
+ *   dense   (ptr NULL) ``segments`` segments of ``length`` rows each; row r of
+ *           segment s at x + s * seg_stride + r * row_stride (elements);
+ *   ragged  ``ptr`` (device int64 [segments + 1], non-decreasing) into
+ *           ``length`` rows of pitch row_stride; segment s = rows [ptr[s],
+ *           ptr[s + 1]).  A segment may be empty; rows outside [ptr[0],
+ *           ptr[segments]) belong to none: their y and grad_x are 0 and they
+ *           add nothing to grad_weight / grad_bias.  Offsets are clamped to
+ *           [0, length], so a bad ptr gives wrong numbers, never an access
+ *           outside the rows.
+ * x, y: GFD_DTYPE_F32 / BF16 / F16, channels contiguous; y (and grad_y /
+ * grad_x) contiguous in the rows' order.  weight / bias [channels], nullable
+ * (identity), w_dtype F32 or x's.  Statistics and sums are fp64; stats (fp64
+ * [segments, groups, 2] = mean, 1/sqrt(var + eps)) is nullable in the forward
+ * and what the backward takes.  channels <= 2048 and a multiple of groups.
+ * GELU is the erf form.  relu's side is decided in fp64 where fp32 cannot
+ * tell it.  grad_weight / grad_bias (w_dtype, nullable) are deterministic.
+ * ws: gfd_group_norm_workspace_size bytes (may be 0: ws may then be NULL).
+ * ------------------------------------------------------------------------- */
+#define GFD_ACT_NONE 0
+#define GFD_ACT_RELU 1
+#define GFD_ACT_SILU 2
+#define GFD_ACT_GELU 3
+size_t gfd_group_norm_workspace_size(int64_t segments, int64_t length, int ragged, int channels,
+                                     int groups, int backward);
+gfd_status gfd_group_norm_fwd(const void* x, int dtype, int64_t segments, int64_t length,
+                              const int64_t* ptr, int channels, int groups, int64_t row_stride,
+                              int64_t seg_stride, const void* weight, const void* bias,
+                              int w_dtype, double eps, int act, void* y, double* stats, void* ws,
+                              size_t ws_bytes, gfd_stream_t stream);
+gfd_status gfd_group_norm_bwd(const void* x, int dtype, int64_t segments, int64_t length,
+                              const int64_t* ptr, int channels, int groups, int64_t row_stride,
+                              int64_t seg_stride, const void* weight, const void* bias,
+                              int w_dtype, int act, const double* stats, const void* grad_y,
+                              void* grad_x, void* grad_weight, void* grad_bias, void* ws,
+                              size_t ws_bytes, gfd_stream_t stream);
+
+/* ---------------------------------------------------------------------------
+ * Log probabilities of given classes with entropy and top alternatives, one
+ * pass over the logits of a classification head (rows of ``classes`` logits,
+ * pitch row_stride elements, F32 / BF16 / F16):
+ *   logp[r]    = x[r, target[r]] - lse_r,  lse = max + log sum exp(x - max)
+ *   entropy[r] = -sum_c p_c log p_c  (natural log; p_c = 0 adds 0)
+ *   top_class[r, 0..top) = the classes of the ``top`` largest logits, larger
+ *                first, equal logits by the lower class;
+ *   top_logp   = their log probabilities.
+ * target (device int64 [rows], nullable together with logp): ignore_index
+ * gives logp 0; any other value outside [0, classes) gives NaN, and reads
+ * nothing.  A masked class is a logit of -inf; a row with nothing else has logp
+ * -inf, entropy 0 and a gradient of 0.  A row with a NaN or +inf logit is NaN
+ * throughout; of a row with a NaN the listed classes are some of its classes.
+ * stats [rows, 2] = (max, log sum exp(x - max)) is what the backward takes.
+ * gfd_class_logp_bwd, with G = grad_logp + sum_j grad_top_j (each gradient
+ * nullable = 0; an ignored row's grad_logp counts as 0):
+ *   grad_logits_c = -p_c (G + grad_entropy (log p_c + entropy))
+ *                   + [c = target] grad_logp + sum_j [c = top_class_j] grad_top_j
+ * contiguous [rows, classes], the logits' type.  0 <= top <= 64, top <= classes
+ * < 2^31.  Deterministic.
+ * ------------------------------------------------------------------------- */
+size_t gfd_class_logp_workspace_size(int64_t rows, int64_t classes, int top);
+gfd_status gfd_class_logp_fwd(const void* logits, int dtype, int64_t rows, int64_t classes,
+                              int64_t row_stride, const int64_t* target, int64_t ignore_index,
+                              int top, float* logp, float* entropy, float* top_logp,
+                              int64_t* top_class, float* stats, void* ws, size_t ws_bytes,
+                              gfd_stream_t stream);
+gfd_status gfd_class_logp_bwd(const void* logits, int dtype, int64_t rows, int64_t classes,
+                              int64_t row_stride, const int64_t* target, int64_t ignore_index,
+                              int top, const int64_t* top_class, const float* stats,
+                              const float* entropy, const float* grad_logp,
+                              const float* grad_entropy, const float* grad_top,
+                              void* grad_logits, gfd_stream_t stream);
+
+/* ---------------------------------------------------------------------------
+ * One Adam / AdamW step over many tensors at once (the optimizer the reference
+ * trains with, train.py:353: Adam, lr 1e-3, weight decay 5e-4):
+ *   g += weight_decay * p                (decoupled 0: Adam)
+ *   p -= lr * weight_decay * p           (decoupled 1: AdamW)
+ *   m = beta1 m + (1 - beta1) g,  v = beta2 v + (1 - beta2) g^2,  t = step + 1
+ *   p -= lr / (1 - beta1^t) * m / (sqrt(v) / sqrt(1 - beta2^t) + eps)
+ * params and grads have one dtype (F32 / BF16 / F16); the arithmetic is fp32
+ * and the parameter is rounded once.  The states live in flat device buffers:
+ * tensor i owns the elements [first, first + numel), first a multiple of 256,
+ * and step[slot], its own step count (device int32), which the call advances --
+ * no argument changes from step to step, so a captured call replays as a real
+ * step.  ``tensors`` is a HOST array (copied into the launch).  Elements must not
+ * overlap between tensors.
+ * state_bits 32: exp_avg (m) and exp_avg_sq (v) are fp32, the scales NULL.
+ * state_bits 8: exp_avg and exp_avg_sq hold e4m3 codes (OCP, 1 byte) of m and of
+ * sqrt(v), each over a power-of-two scale per 256 elements (exp_avg_scale /
+ * exp_avg_sq_scale[element / 256], fp32) chosen so that the block's largest
+ * magnitude over it lies in [128, 256).  The new moments are found in fp64 and
+ * rounded to fp32, then to a code stochastically: with 16 random bits u, a
+ * magnitude a between neighbouring codes q and q' becomes q' iff the fraction
+ * (a - q) / (q' - q) + u / 65536 reaches 1 -- round-to-nearest would leave a
+ * moving average whose step is under half a code where it is.  A non-zero
+ * sqrt(v) never becomes 0.  NaN and infinities become the NaN code.  The random
+ * bits are a hash of (seed, t, element), the lower half for m, the upper for
+ * sqrt(v).
+ * lr_device (nullable): the learning rate as a device float, read by the
+ * kernel, instead of ``lr``.  ticket: one device uint32, 0 before the first call
+ * and 0 again after each; calls that share one must not overlap.
+ * ------------------------------------------------------------------------- */
+typedef struct gfd_adam_tensor {
+  void* param;
+  const void* grad;
+  int64_t numel;
+  int64_t first; /* its first element in the flat states, a multiple of 256 */
+  int64_t slot;  /* its entry in ``step`` */
+} gfd_adam_tensor;
+gfd_status gfd_adam_step(const gfd_adam_tensor* tensors, int64_t num_tensors, int dtype,
+                         int state_bits, void* exp_avg, void* exp_avg_sq, float* exp_avg_scale,
+                         float* exp_avg_sq_scale, int32_t* step, double lr,
+                         const float* lr_device, double beta1, double beta2, double eps,
+                         double weight_decay, int decoupled, uint32_t seed, uint32_t* ticket,
+                         gfd_stream_t stream);
 
 #ifdef __cplusplus
 }
