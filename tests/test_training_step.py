@@ -1,0 +1,239 @@
+"""The operators of a training step together: a GAT with group norms scored by
+class log probabilities with an entropy bonus, its backward, and an Adam / AdamW
+step -- against the fp64 oracle's model, and captured into a graph."""
+import pytest
+import torch
+import torch.nn.functional as F
+
+from _util import assert_close, assert_close_scaled
+
+DEV = "cuda"
+N, E, WIDTH, CLASSES = 1500, 6000, 37, 5
+
+
+def _problem(seed=0):
+    g = torch.Generator().manual_seed(seed)
+    ei = torch.randint(N, (2, E), generator=g)
+    x = torch.randn(N, WIDTH, generator=g)
+    y = torch.randint(CLASSES, (N,), generator=g)
+    y[torch.rand(N, generator=g) < 0.3] = -1
+    return ei, x, y
+
+
+def _model(kind="GAT", **kw):
+    from gfd import models
+    torch.manual_seed(2)
+    m = getattr(models, kind)(WIDTH, 64, CLASSES, num_layers=2, dropout=0.0, norm="group", num_groups=8, **kw)
+    with torch.no_grad():
+        for norm in m.group_norms:
+            norm.weight.uniform_(0.5, 1.5)
+            norm.bias.uniform_(-0.2, 0.2)
+    return m
+
+
+def _oracle_loss(m, ei, x, y):
+    """The same model and loss in fp64 from the oracle's GATConv; parameters by name."""
+    from oracle import gatconv_ref as ref
+    p = {k: v.detach().cpu().double().requires_grad_() for k, v in m.named_parameters()}
+    h = x.double()
+    for li in range(2):
+        c = f"gat_layers.{li}."
+        z = ref.gatconv_forward(h, ei, p[c + "lin_src.weight"], p[c + "att_src"], p[c + "att_dst"], p[c + "bias"])
+        z = F.group_norm(z, 8, p[f"group_norms.{li}.weight"], p[f"group_norms.{li}.bias"]).relu()
+        h = h + z if h.shape == z.shape else z
+    logits = h @ p["out.weight"].t() + p["out.bias"]
+    logp = torch.log_softmax(logits, 1)
+    known = y >= 0
+    loss = -logp[known].gather(1, y[known][:, None]).sum() / known.sum()
+    entropy = -(logp.exp() * logp).sum(1)
+    return loss - 0.05 * entropy.mean(), p, logits.detach()
+
+
+def _loss(m, ei, x, y):
+    r = m.log_probs(x, ei, y, top=2)
+    return -r.log_prob.sum() / (y >= 0).sum() - 0.05 * r.entropy.mean(), r
+
+
+@pytest.mark.gpu
+def test_step_against_the_oracle():
+    from gfd.optim import AdamW
+    ei, x, y = _problem()
+    m = _model().to(DEV).train()
+    loss, r = _loss(m, ei.to(DEV), x.to(DEV), y.to(DEV))
+    loss.backward()
+    ref, p, logits = _oracle_loss(m, ei, x, y)
+    ref.backward()
+    assert abs(loss.item() - ref.item()) <= 1e-5 * abs(ref.item())
+    sure = logits.sort(1, descending=True).values[:, :3].diff(dim=1).abs().min(1).values > 1e-3
+    assert torch.equal(r.top_classes.cpu()[sure], logits.topk(2, 1).indices[sure])
+    for k, v in m.named_parameters():
+        # a gradient's fp32 sums against fp64: 2e-4 of its largest, and what is 0 up to noise
+        assert_close_scaled(v.grad, p[k].grad, rtol=2e-4, atol=1e-7, what=k)
+    # the step itself, on the device's own gradients
+    theirs = [v.detach().cpu().double().requires_grad_() for v in m.parameters()]
+    for a, v in zip(theirs, m.parameters()):
+        a.grad = v.grad.cpu().double()
+    opt, topt = AdamW(m.parameters(), lr=1e-2), torch.optim.AdamW(theirs, lr=1e-2)
+    opt.step()
+    topt.step()
+    for a, v in zip(theirs, m.parameters()):
+        # 16 U of the update (lr) and of the parameter, and its rounding
+        assert (v.detach().cpu().double() - a.detach()).abs().max() <= 20 * 2.0 ** -24 * (1e-2 + a.abs().max())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("kind", ["GAT", "TemporalGNN"])
+@pytest.mark.parametrize("bits", [32, 8])
+def test_training_runs(kind, bits):
+    from gfd.optim import Adam
+    ei, x, y = (t.to(DEV) for t in _problem())
+    m = _model(kind).to(DEV).train()
+    opt = Adam(m.parameters(), lr=1e-3, weight_decay=5e-4, state_bits=bits)
+    before = [p.detach().clone() for p in m.parameters()]
+    for _ in range(3):
+        opt.zero_grad()
+        loss, _ = _loss(m, ei, x, y)
+        loss.backward()
+        opt.step()
+    assert torch.isfinite(loss)
+    for a, p in zip(before, m.parameters()):
+        assert p.isfinite().all() and (p.grad is None or not torch.equal(a, p) or not p.grad.any())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("kind", ["GAT", "TemporalGNN"])
+def test_snapshots_in_training_equal_their_own_passes(kind):
+    """A node's statistics are its own row's: the step-by-step graphs of a temporal graph and
+    the whole give the same in training mode, which batch statistics do not."""
+    ei, x, _ = _problem()
+    step = torch.arange(N) * 3 // N
+    ei = ei[:, step[ei[0]] == step[ei[1]]]
+    m = _model(kind).to(DEV).train()
+    whole = m(x.to(DEV), ei.to(DEV))
+    whole = whole[0] if isinstance(whole, tuple) else whole
+    for s in range(3):
+        at = (step == s).nonzero()[:, 0]
+        sub = ei[:, step[ei[0]] == s] - at[0]
+        part = m(x[at].to(DEV), sub.contiguous().to(DEV))
+        part = part[0] if isinstance(part, tuple) else part
+        assert_close(part, whole[at.to(DEV)].detach(), what=f"step {s}")
+
+
+@pytest.mark.gpu
+def test_eval_equals_training_mode_and_no_grad():
+    ei, x, y = (t.to(DEV) for t in _problem())
+    m = _model().to(DEV)
+    a = m.train()(x, ei)
+    with torch.no_grad():
+        b = m.eval()(x, ei)
+        r = m.log_probs(x, ei, y, top=1)
+    assert_close(b, a.detach(), what="eval")
+    assert torch.equal(r.top_classes[:, 0], b.argmax(1))
+
+
+@pytest.mark.gpu
+def test_rows_scores_and_step_captured_together():
+    """A head over frozen features: norm, scores, gradients and step in one graph, replayed
+    with eager steps of a second copy between."""
+    from gfd.fused import class_log_probs, group_norm
+    from gfd.optim import AdamW
+    gen = torch.Generator().manual_seed(5)
+    x = torch.randn(900, 64, generator=gen).to(DEV)
+    y = torch.randint(-1, CLASSES, (900,), generator=gen).to(DEV)
+    start = [torch.randn(s, generator=gen).to(DEV) * 0.1 for s in ((64,), (64,), (CLASSES, 64))]
+
+    def make():
+        params = [p.clone().requires_grad_() for p in start]
+        opt = AdamW(params, lr=1e-2, state_bits=8, seed=4)
+        for p in params:
+            p.grad = torch.zeros_like(p)
+
+        def step():
+            leaves = [p.detach().requires_grad_() for p in params]
+            h = group_norm(x, 8, leaves[0] + 1, leaves[1], act="silu")
+            r = class_log_probs(h @ leaves[2].t(), y)
+            loss = -r.log_prob.mean() - 0.01 * r.entropy.mean()
+            for p, g in zip(params, torch.autograd.grad(loss, leaves)):
+                p.grad.copy_(g)
+            opt.step()
+        return params, step
+
+    (a, captured), (b, eager) = make(), make()
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        captured()
+    torch.cuda.current_stream().wait_stream(side)
+    eager()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        captured()
+    for _ in range(3):
+        graph.replay()
+        eager()
+        torch.cuda.synchronize()
+        for p, q in zip(a, b):
+            # the head's product and the means are the library's: their order may differ in a graph
+            assert_close_scaled(p, q, rtol=1e-3)
+
+
+def _sharded_rank(rank, world, path, q):
+    import torch.distributed as dist
+    from gfd import dist as gdist, graph as ggraph
+    dist.init_process_group("gloo", init_method=f"file://{path}", rank=rank, world_size=world)
+    try:
+        ei, x, y = _problem()
+        m = _model().to(DEV).train()
+        g = ggraph.csr_from_coo(ei.to(DEV), N)
+        spec = gdist.ShardSpec(g.rowptr.long(), rank, world, "cost")
+        lo, hi = spec.dst_lo, spec.dst_hi
+        rp = g.rowptr.long()
+        plan = gdist.HaloPlan.create(g.col[int(rp[lo]):int(rp[hi])], spec)
+        logits = gdist.gat_forward_sharded_train(m, x.to(DEV), gdist.local_graph(g, lo, hi), plan, N)
+        from gfd.fused import class_log_probs
+        r = class_log_probs(logits, y[lo:hi].to(DEV))
+        (-r.log_prob.sum() / int((y >= 0).sum()) - 0.05 * r.entropy.sum() / N).backward()
+        gdist.all_reduce_grads(list(m.parameters()))
+        if rank == 0:
+            q.put({k: p.grad.cpu().numpy() for k, p in m.named_parameters()})
+        dist.barrier()
+    finally:
+        dist.destroy_process_group()
+
+
+@pytest.mark.gpu
+def test_sharded_step_needs_no_exchange_for_the_norm():
+    import torch.multiprocessing as mp
+    from test_dist_cpu import _store_path
+    ctx = mp.get_context("spawn")
+    q, path = ctx.Queue(), _store_path()
+    procs = [ctx.Process(target=_sharded_rank, args=(r, 2, path, q)) for r in range(2)]
+    for p in procs:
+        p.start()
+    got = q.get(timeout=100)
+    for p in procs:
+        p.join(timeout=60)
+        assert p.exitcode == 0
+    ei, x, y = _problem()
+    ref, p, _ = _oracle_loss(_model(), ei, x, y)
+    ref.backward()
+    for k, g in got.items():
+        assert_close_scaled(torch.from_numpy(g), p[k].grad, rtol=2e-4, atol=1e-7, what=k)
+
+
+def test_norm_argument_and_state_dict_keys():
+    from gfd.models import GAT, TemporalGNN
+    with pytest.raises(ValueError, match="norm must be"):
+        GAT(8, 64, 2, norm="layer")
+    with pytest.raises(ValueError, match="divisible"):
+        GAT(8, 64, 2, norm="group", num_groups=7)
+    assert not any("group_norms" in k for k in GAT(8, 64, 2).state_dict())
+    keys = TemporalGNN(8, 64, 2, norm="group").state_dict()
+    assert "group_norms.1.weight" in keys and not any("batch_norms" in k for k in keys)
+
+
+def test_sharded_inference_refuses_group_norms():
+    from gfd import dist as gdist
+    m = _model().eval()
+    with torch.no_grad(), pytest.raises(NotImplementedError, match="norm='group'"):
+        gdist.model_forward_sharded(m, None, None, None)
