@@ -22,7 +22,8 @@ train.py:143): the same constructor arguments and update, over
 """
 from __future__ import annotations
 
-from typing import Dict, List
+from operator import attrgetter
+from typing import Dict, Tuple
 
 import numpy as np
 import torch
@@ -32,6 +33,12 @@ from . import _lib
 STATE_BLOCK = 256
 _CODES = {torch.float32: _lib.DTYPE_F32, torch.bfloat16: _lib.DTYPE_BF16,
           torch.float16: _lib.DTYPE_F16}
+
+
+_grad, _dtype, _layout = attrgetter("grad"), attrgetter("dtype"), attrgetter("layout")
+_data_ptr, _numel, _device, _contiguous = (torch.Tensor.data_ptr, torch.Tensor.numel,
+                                           torch.Tensor.get_device, torch.Tensor.is_contiguous)
+_NONE = type(None)
 
 
 def _dense(p: torch.Tensor) -> bool:
@@ -121,7 +128,7 @@ class Adam(torch.optim.Optimizer):
             total += -(-p.numel() // STATE_BLOCK) * STATE_BLOCK
         f = {"first": first, "numel": [p.numel() for p in params], "bits": self.param_groups[gi]["state_bits"], "device": dev,
              "step": torch.zeros(len(params), dtype=torch.int32, device=dev),
-             "ticket": torch.zeros(1, dtype=torch.int32, device=dev)}
+             "ticket": torch.zeros(1056, dtype=torch.int32, device=dev)}
         if f["bits"] == 32:
             f["exp_avg"] = torch.zeros(total, dtype=torch.float32, device=dev)
             f["exp_avg_sq"] = torch.zeros(total, dtype=torch.float32, device=dev)
@@ -129,6 +136,9 @@ class Adam(torch.optim.Optimizer):
             for k in ("exp_avg", "exp_avg_sq"):
                 f[k] = torch.zeros(total, dtype=torch.uint8, device=dev).view(torch.float8_e4m3fn)
                 f[k + "_scale"] = torch.zeros(total // STATE_BLOCK, dtype=torch.float32, device=dev)
+        # gfd_adam_tensor of every parameter; the two pointers are filled in at each step
+        f["table"] = np.array([(0, 0, p.numel(), at, i) for i, (p, at) in enumerate(zip(params, first))],
+                              dtype=np.int64)
         self._flat[gi] = f
         for i, p in enumerate(params):
             self.state[p] = self._views(f, i, p)
@@ -211,52 +221,84 @@ class Adam(torch.optim.Optimizer):
         return loss
 
     def _step_group(self, group: dict, f: dict) -> None:
-        dev, first, numel = f["device"], f["first"], f["numel"]
-        tables: Dict[torch.dtype, List[int]] = {}
+        params = group["params"]
+        grads = list(map(_grad, params))
+        index, numel = f["device"].index, f["numel"]
+        dtype, n = params[0].dtype, len(params)
+        # the ordinary step, looked over a property at a time: every gradient there, dense and
+        # contiguous like its parameter, one type, the device and sizes that the states were made for
+        if (_NONE not in map(type, grads) and
+                list(map(_dtype, params)).count(dtype) == n == list(map(_dtype, grads)).count(dtype) and
+                list(map(_layout, grads)).count(torch.strided) == n and
+                list(map(_device, params)).count(index) == n == list(map(_device, grads)).count(index) and
+                list(map(_numel, params)) == numel == list(map(_numel, grads)) and
+                all(map(_contiguous, params)) and all(map(_contiguous, grads))):
+            table = f["table"]
+            table[:, 0] = list(map(_data_ptr, params))
+            table[:, 1] = list(map(_data_ptr, grads))
+            self._launch(group, f, dtype, table)
+            return
+        self._step_mixed(group, f)
+
+    def _step_mixed(self, group: dict, f: dict) -> None:
+        """A step whose gradients are missing in part, of several types or in other orders
+        than their parameters'; says what is wrong with one that cannot be taken."""
+        dev, numel = f["device"], f["numel"]
+        index = dev.index
+        tables: Dict[torch.dtype, Tuple[list, list, list]] = {}
         kept = []                       # copies of gradients, alive until the launch is queued
+        dtype = params = grads = places = None
         for i, p in enumerate(group["params"]):
             g = p.grad
             if g is None:
                 continue
-            dtype = p.dtype
-            if g.dtype != dtype or g.is_sparse or g.device != dev or p.device != dev:
+            if p.dtype is not dtype:
+                dtype = p.dtype
+                params, grads, places = tables.setdefault(dtype, ([], [], []))
+            if (g.dtype is not dtype or g.is_sparse or g.get_device() != index or
+                    p.get_device() != index):
                 raise RuntimeError(f"gfd Adam: a gradient must be dense, {dtype} and on {dev} like its "
                                    f"parameter (got {g.layout}, {g.dtype}, {g.device})")
-            if p.numel() != numel[i]:
-                raise RuntimeError(f"gfd Adam: a parameter changed its size from {numel[i]} to "
-                                   f"{p.numel()}")
+            n = numel[i]
+            if p.numel() != n or g.numel() != n:
+                raise RuntimeError(f"gfd Adam: a parameter changed its size from {n} to {p.numel()}")
             if not (p.is_contiguous() and g.is_contiguous()) and g.stride() != p.stride():
                 g = torch.empty_like(p).copy_(g)
                 kept.append(g)
-            tables.setdefault(dtype, []).extend(
-                (p.data_ptr(), g.data_ptr(), numel[i], first[i], i))
-        lr = group["lr"]
-        lr_ptr = None
+            params.append(p.data_ptr())
+            grads.append(g.data_ptr())
+            places.append(i)
+        for dtype, (params, grads, places) in tables.items():
+            table = f["table"][places]
+            table[:, 0] = params
+            table[:, 1] = grads
+            self._launch(group, f, dtype, table)
+
+    def _launch(self, group: dict, f: dict, dtype: torch.dtype, table: np.ndarray) -> None:
+        dev, lr, lr_ptr = f["device"], group["lr"], None
         if isinstance(lr, torch.Tensor):
             if lr.device != dev:
                 raise RuntimeError(f"gfd Adam: lr is on {lr.device}, expected {dev}")
             lr, lr_ptr = 0.0, lr.data_ptr()
         b1, b2 = group["betas"]
-        for dtype, flat in tables.items():
-            table = np.array(flat, dtype=np.int64)
-            _check_apart(table.reshape(-1, 5), dtype.itemsize)
-            _lib.call_on(dev, "gfd_adam_step", table.ctypes.data, table.size // 5, _CODES[dtype],
-                         f["bits"], f["exp_avg"].data_ptr(), f["exp_avg_sq"].data_ptr(),
-                         _lib.ptr(f.get("exp_avg_scale")), _lib.ptr(f.get("exp_avg_sq_scale")),
-                         f["step"].data_ptr(), float(lr), lr_ptr, float(b1), float(b2),
-                         float(group["eps"]), float(group["weight_decay"]),
-                         1 if self._decoupled else 0, int(group["seed"]), f["ticket"].data_ptr(),
-                         _lib.stream_handle(dev))
+        _check_apart(table, dtype.itemsize)
+        _lib.call_on(dev, "gfd_adam_step", table.ctypes.data, len(table), _CODES[dtype], f["bits"],
+                     f["exp_avg"].data_ptr(), f["exp_avg_sq"].data_ptr(),
+                     _lib.ptr(f.get("exp_avg_scale")), _lib.ptr(f.get("exp_avg_sq_scale")),
+                     f["step"].data_ptr(), float(lr), lr_ptr, float(b1), float(b2),
+                     float(group["eps"]), float(group["weight_decay"]), 1 if self._decoupled else 0,
+                     int(group["seed"]), f["ticket"].data_ptr(), _lib.stream_handle(dev))
 
 
 def _check_apart(table: np.ndarray, itemsize: int) -> None:
     """Refuse parameters that share memory: one launch updates all of them."""
-    table = table[table[:, 2] > 0]
-    order = np.argsort(table[:, 0], kind="stable")
-    begin = table[order, 0]
-    end = begin + table[order, 2] * itemsize
-    if (end[:-1] > begin[1:]).any():
-        raise ValueError("gfd Adam: two parameters share memory")
+    begin, size = table[:, 0], table[:, 2] * itemsize
+    if size.size > 1 and ((begin[1:] < begin[:-1] + size[:-1]) | (size[1:] == 0)).any():
+        # not in the order of their addresses
+        order = np.argsort(begin[size > 0], kind="stable")
+        begin, size = begin[size > 0][order], size[size > 0][order]
+        if (begin[1:] < begin[:-1] + size[:-1]).any():
+            raise ValueError("gfd Adam: two parameters share memory")
 
 
 class AdamW(Adam):

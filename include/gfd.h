@@ -686,9 +686,10 @@ gfd_status gfd_class_logp_bwd(const void* logits, int dtype, int64_t rows, int64
  * bits are a hash of (seed, t, element), the lower half for m, the upper for
  * sqrt(v).
  * lr_device (nullable): the learning rate as a device float, read by the
- * kernel, instead of ``lr``.  ticket: one device uint32, 0 before the first call
- * and 0 again after each; calls that share one must not overlap.
+ * kernel, instead of ``lr``.  ticket: GFD_ADAM_TICKETS device uint32, 0 before
+ * the first call and 0 again after each; calls that share them must not overlap.
  * ------------------------------------------------------------------------- */
+#define GFD_ADAM_TICKETS 1056
 typedef struct gfd_adam_tensor {
   void* param;
   const void* grad;
