@@ -15,7 +15,8 @@
 //     iteration.
 //   * The top list is a wave's: entry j in lane j.  A vector of logits enters the
 //     search only where its largest is above the list's last entry, the same
-//     comparison as the reference's.
+//     comparison as the reference's; the waves that share a row tell each other
+//     their lists' last entries.
 // Rows of up to kNarrow classes are read by teams of 1 to 32 lanes, longer ones
 // by a wave, long ones by a block; few long rows are split over blocks whose
 // partial results a second kernel joins.
@@ -35,7 +36,6 @@ constexpr int kFill = 1024;        // blocks that fill the card: rows are split 
 constexpr float kSlack = 8.f;
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kInf = __builtin_inff();
-constexpr int kNone = INT32_MIN;   // below the key of every logit
 
 __device__ __forceinline__ float exp_of(float d) { return __builtin_amdgcn_exp2f(d * kLog2e); }
 
@@ -51,30 +51,31 @@ __device__ __forceinline__ float max3_f(float a, float b, float c) {
   return r;
 }
 
-// int32 that orders like the logit; -0 as +0, NaN as -inf
-__device__ __forceinline__ int key_of(float x) {
-  x = x == x ? x + 0.f : -kInf;
-  const int b = __float_as_int(x);
-  return b < 0 ? b ^ 0x7FFFFFFF : b;
-}
-__device__ __forceinline__ float value_of(int key) {
-  return __int_as_float(key < 0 ? key ^ 0x7FFFFFFF : key);
-}
-
+// reductions over the wave, uniform: lane 15 of a row of 16 collects its row's, rows 1 and 3
+// the row before, rows 2 and 3 the first two; lanes without a source read ``none``
 template <int CTRL, int ROWS>
-__device__ __forceinline__ int dpp_max(int v) {
-  const int o = __builtin_amdgcn_update_dpp(kNone, v, CTRL, ROWS, 0xF, false);
-  return v > o ? v : o;
+__device__ __forceinline__ float dpp(float none, float v) {
+  return __int_as_float(__builtin_amdgcn_update_dpp(__float_as_int(none), __float_as_int(v), CTRL, ROWS, 0xF, false));
 }
-// max over the wave, in every lane
-__device__ __forceinline__ int wave_max(int v) {
-  v = dpp_max<0x111, 0xF>(v);  // row_shr 1, 2, 4, 8: lane 15 of a row holds its row's
-  v = dpp_max<0x112, 0xF>(v);
-  v = dpp_max<0x114, 0xF>(v);
-  v = dpp_max<0x118, 0xF>(v);
-  v = dpp_max<0x142, 0xA>(v);  // row_bcast 15 into rows 1 and 3
-  v = dpp_max<0x143, 0xC>(v);  // row_bcast 31 into rows 2 and 3
-  return __builtin_amdgcn_readlane(v, 63);
+template <typename F>
+__device__ __forceinline__ float wave_reduce(float none, float v, F f) {
+  v = f(v, dpp<0x111, 0xF>(none, v));  // row_shr 1, 2, 4, 8
+  v = f(v, dpp<0x112, 0xF>(none, v));
+  v = f(v, dpp<0x114, 0xF>(none, v));
+  v = f(v, dpp<0x118, 0xF>(none, v));
+  v = f(v, dpp<0x142, 0xA>(none, v));  // row_bcast 15, 31
+  v = f(v, dpp<0x143, 0xC>(none, v));
+  return __int_as_float(__builtin_amdgcn_readlane(__float_as_int(v), 63));
+}
+// the largest that is not NaN
+__device__ __forceinline__ float wave_max(float v) {
+  return wave_reduce(-kInf, v, [](float a, float b) { return max_f(a, b); });
+}
+__device__ __forceinline__ float wave_sum(float v) {
+  return wave_reduce(0.f, v, [](float a, float b) { return a + b; });
+}
+__device__ __forceinline__ float lane_of(float v, int lane) {
+  return __int_as_float(__builtin_amdgcn_readlane(__float_as_int(v), lane));
 }
 template <int W>
 __device__ __forceinline__ float team_sum(float v) {
@@ -94,69 +95,118 @@ struct Sums {
     s *= f;
     r = to;
   }
-  __device__ __forceinline__ void add(float x) {
-    const float d = x - (r == -kInf ? 0.f : r);
+  __device__ __forceinline__ void add(float x) { add_about(x, r == -kInf ? 0.f : r); }
+  __device__ __forceinline__ void add_about(float x, float about) {
+    const float d = x - about;
     const float e = exp_of(d);
     s += e;
     t = fmaf(e, max_f(d, -1000.f), t);  // e = 0 at d = -inf: adds 0
   }
-  // the team's sums, in every lane of it
-  template <int W>
+  // the wave's sums, in every lane of it
   __device__ __forceinline__ void join() {
-    float to = r;
-#pragma unroll
-    for (int d = 1; d < W; d <<= 1) to = max_f(to, __shfl_xor(to, d, W));
+    const float to = wave_max(r);
     if (to != -kInf) move(to);
-    s = team_sum<W>(s);
-    t = team_sum<W>(t);
+    s = wave_sum(s);
+    t = wave_sum(t);
   }
 };
 
 // a wave's list of the largest logits so far, larger first, equal ones by the
-// lower class; entry j in lane j
+// lower class; entry j in lane j, lanes from ``size`` on NaN
+__device__ __forceinline__ float above(float v) {  // the next float
+  const uint32_t b = __float_as_uint(v);
+  return __uint_as_float(v == 0.f ? 1u : v > 0.f ? b + 1 : b - 1);
+}
+__device__ __forceinline__ float below(float v) { return -above(-v); }
+
 struct Top {
-  int key = kNone;
+  float val = __builtin_nanf("");
   int cls = 0;
-  int size = 0;   // uniform
-  float floor = -kInf;  // the last entry of a full list
-  __device__ __forceinline__ void put(int k, int c, int top) {
+  int size = 0;                     // uniform
+  float floor = -kInf;              // of a full list, uniform: its last entry
+  int floor_cls = INT32_MAX;
+
+  __device__ __forceinline__ void put(float v, int c, int top) {
     const int lane = threadIdx.x & 63;
-    const int at = __popcll(__ballot(lane < size && (key > k || (key == k && cls < c))));
-    const int up_k = __shfl_up(key, 1), up_c = __shfl_up(cls, 1);
-    if (lane > at) {
-      key = up_k;
-      cls = up_c;
-    } else if (lane == at) {
-      key = k;
-      cls = c;
-    }
+    const int at = __popcll(__ballot(val > v || (val == v && cls < c)));
+    // wave_shr 1: the entry of the lane before
+    const float up = dpp<0x138, 0xF>(val, val);
+    const int up_c = __builtin_amdgcn_update_dpp(cls, cls, 0x138, 0xF, 0xF, false);
+    val = lane > at ? up : lane == at ? v : val;
+    cls = lane > at ? up_c : lane == at ? c : cls;
+    val = lane < top ? val : __builtin_nanf("");
     size = size < top ? size + 1 : top;
-    if (size == top) floor = value_of(__builtin_amdgcn_readlane(key, top - 1));
+    if (size == top) {
+      floor = lane_of(val, top - 1);
+      floor_cls = __builtin_amdgcn_readlane(cls, top - 1);
+    }
   }
-  // N logits a lane, the class of lane l's j-th is base + l * N + j; those outside
-  // [0, classes) are none.  Later calls have higher classes.
-  template <int N>
-  __device__ void take(const float (&x)[N], int base, int classes, int top) {
-    int k[N];
-    const int lane = threadIdx.x & 63;
-    const int c0 = base + lane * N;
+
+  // A bound from below of the ``top``-th largest of the lanes' values (NaN: none), of which
+  // about that many are not below it: the upper half of its bits, found one by one
+  __device__ __forceinline__ static float bound_of(float v, int top) {
+    if (__popcll(__ballot(v == v)) < top) return -kInf;
+    const uint32_t b = __float_as_uint(v + 0.f);
+    // unsigned bits that order like the values
+    const uint32_t u = v == v ? (b & 0x80000000u ? ~b : b | 0x80000000u) : 0u;
+    uint32_t low = 0;
+#pragma unroll 1
+    for (uint32_t bit = 1u << 31; bit >= 1u << 16; bit >>= 1)
+      if (__popcll(__ballot(u >= (low | bit))) >= top) low |= bit;
+    if (low < 0x00800000u) return -kInf;  // -inf, or what would be a NaN's bits
+    return __uint_as_float(low & 0x80000000u ? low & 0x7FFFFFFFu : ~low);
+  }
+
+  // would a candidate enter the list
+  __device__ __forceinline__ bool fits(float v, int c, int top) const {
+    return size < top ? v == v : v > floor || (v == floor && c < floor_cls);
+  }
+
+  // a candidate a lane; ``some``: the lanes that have one that fits
+  __device__ __forceinline__ void merge(unsigned long long some, float v, int c, int top) {
+    while (some) {
+      const int l = __ffsll(some) - 1;
+      put(lane_of(v, l), __builtin_amdgcn_readlane(c, l), top);
+      some &= some - 1;
+      if (size == top) some &= __ballot(fits(v, c, top));
+    }
+  }
+
+  // a listed entry a lane, NaN: none
+  __device__ __forceinline__ void join(float v, int c, int top) {
+    const float low = size < top ? bound_of(v, top) : -kInf;
+    merge(__ballot(v >= low && fits(v, c, top)), v, c, top);
+  }
+
+  // The logits x of a wave's vector, ``have`` of a lane's N from class cls0 on, those below
+  // ``least`` not wanted.  They come in the order of their classes, lane by lane, and (ORDERED)
+  // after all lower classes: once the list is full, one that equals its last entry is not.
+  template <bool ORDERED, int N>
+  __device__ __forceinline__ void take(const float (&x)[N], int have, int cls0, int top, float least) {
+    float best = __builtin_nanf("");
 #pragma unroll
-    for (int j = 0; j < N; ++j) k[j] = c0 + j >= 0 && c0 + j < classes ? key_of(x[j]) : kNone;
-    for (;;) {
-      int best = k[0];
+    for (int j = 0; j < N; ++j) best = max_f(best, j < have ? x[j] : __builtin_nanf(""));
+    float low = size < top ? bound_of(best, top) : ORDERED ? above(floor) : floor;
+    low = max_f(low, least);
+    uint32_t bits = 0;
 #pragma unroll
-      for (int j = 1; j < N; ++j) best = best > k[j] ? best : k[j];
-      const int m = wave_max(best);
-      if (m == kNone || (size == top && m <= __builtin_amdgcn_readlane(key, top - 1))) return;
-      const int from = __ffsll((unsigned long long)__ballot(best == m)) - 1;
-      int j0 = 0;
+    for (int j = 0; j < N; ++j) bits |= x[j] >= low ? 1u << j : 0u;
+    bits &= (1u << have) - 1;
+    unsigned long long some = __ballot(bits != 0);
+    while (some) {
+      const int l = __ffsll(some) - 1;
+      uint32_t b = __builtin_amdgcn_readlane(bits, l);
+      const int c0 = __builtin_amdgcn_readlane(cls0, l);
+      for (; b; b &= b - 1) {
+        const int j = __ffs(b) - 1;
+        float v = x[0];
 #pragma unroll
-      for (int j = N - 1; j >= 0; --j) j0 = k[j] == m ? j : j0;
-      const int c = __builtin_amdgcn_readlane(c0 + j0, from);
-#pragma unroll
-      for (int j = 0; j < N; ++j)
-        if (lane == from && j == j0) k[j] = kNone;
-      put(m, c, top);
+        for (int i = 1; i < N; ++i) v = i == j ? x[i] : v;
+        const float m = lane_of(v, l);
+        if (size < top || m > floor || (!ORDERED && m == floor && c0 + j < floor_cls)) put(m, c0 + j, top);
+      }
+      some &= some - 1;
+      if (size == top) some &= __ballot(ORDERED ? best > floor : best >= floor);
     }
   }
 };
@@ -170,8 +220,6 @@ struct RowOut {
   int64_t* top_class;
   float* stats;
 };
-
-__device__ __forceinline__ float log_of(float s) { return __logf(s); }
 
 // log p of a logit from the row's statistics (R, log S); an empty row: -inf
 __device__ __forceinline__ float logp_of(float x, float r, float ls) {
@@ -221,33 +269,36 @@ __global__ void __launch_bounds__(kThreads) k_fwd_narrow(const T* __restrict__ x
     if (l == 0) write_row(o, row, xr, classes, a.r, a.s, a.t);
     if (top) {
       const float ls = a.s == 0.f ? -kInf : logf(a.s);
-      int k[4];
+      // a taken entry, one outside of the classes and NaN are none: NaN
 #pragma unroll
-      for (int j = 0; j < 4; ++j) k[j] = j * W + l < classes ? key_of(v[j]) : kNone;
+      for (int j = 0; j < 4; ++j)
+        if (j * W + l >= classes) v[j] = __builtin_nanf("");
       for (int n = 0; n < top; ++n) {
-        int bk = kNone, bc = INT32_MAX;
+        float bv = __builtin_nanf("");
+        int bc = INT32_MAX;
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-          if (k[j] > bk) {
-            bk = k[j];
+          if (v[j] > bv || (bv != bv && v[j] == v[j])) {
+            bv = v[j];
             bc = j * W + l;
           }
         }
 #pragma unroll
         for (int d = 1; d < W; d <<= 1) {
-          const int ok = __shfl_xor(bk, d, W), oc = __shfl_xor(bc, d, W);
-          if (ok > bk || (ok == bk && oc < bc)) {
-            bk = ok;
+          const float ov = __shfl_xor(bv, d, W);
+          const int oc = __shfl_xor(bc, d, W);
+          if (ov > bv || (ov == bv && oc < bc) || (bv != bv && ov == ov)) {
+            bv = ov;
             bc = oc;
           }
         }
-        if (l == 0) {
-          o.top_class[row * top + n] = bc;
-          o.top_logp[row * top + n] = logp_of(value_of(bk), a.r, ls);
+        if (l == 0) {  // (of a row with a NaN some class: the first)
+          o.top_class[row * top + n] = bv == bv ? bc : 0;
+          o.top_logp[row * top + n] = logp_of(bv, a.r, ls);
         }
 #pragma unroll
         for (int j = 0; j < 4; ++j)
-          if (bc == j * W + l) k[j] = kNone;
+          if (bc == j * W + l) v[j] = __builtin_nanf("");
       }
     }
   }
@@ -256,115 +307,147 @@ __global__ void __launch_bounds__(kThreads) k_fwd_narrow(const T* __restrict__ x
 // ---------------------------------------------------------------------------
 // more classes: W waves of a block a row, or a split of one
 // ---------------------------------------------------------------------------
-struct Partial {  // of a split, followed by its top list
+struct Partial {  // of a wave or a split
   float r, s, t;
-  int size;
 };
 
 // sums and top list of the elements [begin, end) of a row that this wave reads:
-// wave w of W
+// wave w of W.  best_floor (LDS, nullable): the highest floor of the waves' lists, a bound
+// from below of the row's list
 template <typename T, int W>
 __device__ __forceinline__ void scan_row(const T* xr, int begin, int end, int w, int top, Sums& a,
-                                         Top& best) {
+                                         Top& best, volatile float* best_floor) {
   constexpr int V = 16 / sizeof(T);
-  constexpr int U = 4;
+  constexpr int U = 2;  // vectors in flight a lane
   const int lane = threadIdx.x & 63;
   float bound = -kInf;  // a vector whose largest logit is not above it needs no second look
-  auto again = [&]() {
+  float least = -kInf;  // nor is one below this wanted in the list
+  auto limit = [&]() {
     bound = a.r + kSlack;
-    if (top) bound = best.size == top ? (bound < best.floor ? bound : best.floor) : -kInf;
-  };
-  auto one = [&](const auto& x, int base) {  // base: the class of lane 0's first logit
-    constexpr int N = sizeof(x) / sizeof(float);
-    float m = x[0];
-    if constexpr (N > 1) {
-      m = max_f(x[0], x[1]);
-#pragma unroll
-      for (int j = 2; j + 1 < N; j += 2) m = max3_f(m, x[j], x[j + 1]);
+    if (top) {
+      // equal to another wave's floor: wanted, its class may be the lower one
+      const float f = best.size < top ? -kInf : best.floor >= least ? best.floor : below(least);
+      bound = f < bound ? f : bound;
     }
-    if (__ballot(m > bound || (top && best.size < top))) {
-      if (m > a.r + kSlack) a.move(m);
-      if (top && __ballot(m > best.floor || best.size < top)) best.take(x, base, end, top);
-      again();
-    }
-#pragma unroll
-    for (int j = 0; j < N; ++j) a.add(x[j]);
   };
-  // [begin, lo) and [hi, end): what the 16-byte vectors leave, one element a lane
+  // [begin, lo) and [hi, end): what the 16-byte vectors leave, under 16 classes
   const int head = int((16 - (reinterpret_cast<uintptr_t>(xr + begin) & 15)) & 15) / int(sizeof(T));
   const int lo = begin + (head < end - begin ? head : end - begin);
   const int vecs = (end - lo) / V, hi = lo + vecs * V;
-  if (w == 0 && lo > begin) {
-    const float x[1] = {lane < lo - begin ? to_f32(xr[begin + lane]) : -kInf};
-    one(x, lane < lo - begin ? begin : end);
-  }
+  const int rest = w == 0 ? lo - begin + end - hi : 0;
   const auto* p = reinterpret_cast<const Pack<T, V>*>(xr + lo);
-  for (int v0 = w * 64; v0 < vecs; v0 += W * 64 * U) {
+  // groups of U vectors, then the rest as a group of its own
+  for (int v0 = w * 64;; v0 += W * 64 * U) {
+    const bool last = v0 >= vecs;
+    if (last && rest <= 0) break;
     Pack<T, V> q[U];
+    if (v0 + (U - 1) * W * 64 + 64 <= vecs) {
+#pragma unroll
+      for (int u = 0; u < U; ++u) q[u] = p[v0 + u * W * 64 + lane];
+    } else {
+#pragma unroll
+      for (int u = 0; u < U; ++u)
+#pragma unroll
+        for (int j = 0; j < V; ++j) q[u].v[j] = from_f32<T>(-kInf);
+      if (!last) {
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+          if (v0 + u * W * 64 + lane < vecs) q[u] = p[v0 + u * W * 64 + lane];
+      } else if (lane < rest) {  // one element a lane, those before the vectors first
+        q[0].v[0] = xr[lane < lo - begin ? begin + lane : hi + lane - (lo - begin)];
+      }
+    }
+    // vectors of this group that some lane has
+    const int live = last ? 1 : min(U, (vecs - v0 + W * 64 - 1) / (W * 64));
+    if (W > 1 && top) {
+      const float f = *best_floor;
+      if (__ballot(f > least)) {
+        least = f;
+        limit();
+      }
+    }
+    float m[U], all = -kInf;
 #pragma unroll
     for (int u = 0; u < U; ++u) {
-      const int v = v0 + u * W * 64 + lane;
-      if (v < vecs) q[u] = p[v];
+      m[u] = -kInf;
+#pragma unroll
+      for (int j = 0; j < V; j += 2) m[u] = max3_f(m[u], to_f32(q[u].v[j]), to_f32(q[u].v[j + 1]));
+      all = max_f(all, m[u]);
     }
+    if (__ballot(all > bound) || (top && (last || best.size < top))) {
+      if (all > a.r + kSlack) a.move(all);
+      if (top) {
+        uint32_t todo = 0;  // the vectors with something for the list
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+          if (u < live && (last || best.size < top || __ballot(m[u] > best.floor && m[u] >= least)))
+            todo |= 1u << u;
+#pragma unroll 1
+        for (; todo; todo &= todo - 1) {
+          const int u = __ffs(todo) - 1;
+          Pack<T, V> c = q[0];
+#pragma unroll
+          for (int k = 1; k < U; ++k)
+            if (u == k) c = q[k];
+          float y[V];
+#pragma unroll
+          for (int j = 0; j < V; ++j) y[j] = to_f32(c.v[j]);
+          if (!last) {
+            const int v = v0 + u * W * 64 + lane;
+            best.template take<true>(y, v < vecs ? V : 0, lo + v * V, top, least);
+          } else {
+            const float z[1] = {y[0]};
+            best.template take<false>(z, lane < rest ? 1 : 0,
+                                      lane < lo - begin ? begin + lane : hi + lane - (lo - begin), top, least);
+          }
+          if (W > 1 && best.size == top && best.floor > least) *best_floor = least = best.floor;
+        }
+      }
+      limit();
+    }
+    const float r = a.r == -kInf ? 0.f : a.r;
 #pragma unroll
     for (int u = 0; u < U; ++u) {
-      const int v = v0 + u * W * 64;
-      if (v >= vecs) break;
-      float x[V];
+      if (u < live) {
 #pragma unroll
-      for (int j = 0; j < V; ++j) x[j] = v + lane < vecs ? to_f32(q[u].v[j]) : -kInf;
-      // classes beyond hi belong to the tail: none here
-      one(x, v + lane < vecs ? lo + v * V : end);
+        for (int j = 0; j < V; ++j) a.add_about(to_f32(q[u].v[j]), r);
+      }
     }
-  }
-  if (w == 0 && hi < end) {
-    const float x[1] = {lane < end - hi ? to_f32(xr[hi + lane]) : -kInf};
-    one(x, hi);
+    if (last) break;
   }
 }
 
-// the larger first, equal ones by the lower class: the top of ``n`` listed entries
-template <typename F>
-__device__ __forceinline__ void top_of_lists(const int2* list, int n, int top, F put) {
+struct Entry {  // of a list
+  float val;
+  int cls;
+};
+
+// the list of a row, a lane an entry; of a row with a NaN, some classes
+__device__ __forceinline__ void write_top(const RowOut& o, int64_t row, int top, const Top& best,
+                                          float r, float s) {
   const int lane = threadIdx.x & 63;
-  int last_k = INT32_MAX, last_c = -1;
-  for (int out = 0; out < top; ++out) {
-    // the largest entry after the last one put
-    int bk = kNone, bc = INT32_MAX;
-    for (int i = lane; i < n; i += 64) {
-      const int2 e = list[i];
-      const bool after = e.x < last_k || (e.x == last_k && e.y > last_c);
-      if (after && (e.x > bk || (e.x == bk && e.y < bc))) {
-        bk = e.x;
-        bc = e.y;
-      }
-    }
-#pragma unroll
-    for (int d = 1; d < 64; d <<= 1) {
-      const int ok = __shfl_xor(bk, d), oc = __shfl_xor(bc, d);
-      if (ok > bk || (ok == bk && oc < bc)) {
-        bk = ok;
-        bc = oc;
-      }
-    }
-    last_k = bk;
-    last_c = bc;
-    put(out, bk, bc);
+  if (lane < top) {
+    const float ls = s == 0.f ? -kInf : logf(s);
+    o.top_class[row * top + lane] = lane < best.size ? best.cls : 0;
+    o.top_logp[row * top + lane] = logp_of(best.val, r, ls);
   }
 }
 
+// (8 waves a SIMD, 64 registers: with 4 vectors in flight and 5 waves, or the next group read
+// ahead, the kernel is up to 15 % slower)
 template <typename T, int W, bool SPLIT>
-__global__ void __launch_bounds__(kThreads) k_fwd_wide(const T* __restrict__ x, int64_t rows,
+__global__ void __launch_bounds__(kThreads, 8) k_fwd_wide(const T* __restrict__ x, int64_t rows,
                                                        int classes, int64_t stride, int top,
                                                        int splits, int per_split,
                                                        Partial* __restrict__ part,
-                                                       int2* __restrict__ part_top, RowOut o) {
+                                                       Entry* __restrict__ part_top, RowOut o) {
   __shared__ Partial sums[kWaves];
-  __shared__ int2 lists[W > 1 ? W * kMaxTop : 1];
+  __shared__ Entry lists[W > 1 ? W * kMaxTop : 1];
+  __shared__ float best_floor;
   const int lane = threadIdx.x & 63, wave = wave_uniform(threadIdx.x >> 6);
   const int64_t jobs = rows * (SPLIT ? splits : 1);
   const int64_t step = int64_t(gridDim.x) * (kWaves / W);
-  // every wave of a block runs the same number of iterations (a barrier inside)
+  // every wave of a block runs the same number of iterations (barriers inside)
   for (int64_t job0 = int64_t(blockIdx.x) * (kWaves / W); job0 < jobs; job0 += step) {
     const int64_t job = job0 + (W > 1 ? 0 : wave);
     if (W == 1 && job >= jobs) break;
@@ -372,13 +455,17 @@ __global__ void __launch_bounds__(kThreads) k_fwd_wide(const T* __restrict__ x, 
     const int begin = SPLIT ? int(job - row * splits) * per_split : 0;
     const int end = SPLIT ? (begin + per_split < classes ? begin + per_split : classes) : classes;
     const T* xr = x + row * stride;
+    if (W > 1 && top) {
+      if (threadIdx.x == 0) best_floor = -kInf;
+      __syncthreads();
+    }
     Sums a;
     Top best;
-    scan_row<T, W>(xr, begin, end, W > 1 ? wave : 0, top, a, best);
-    a.join<64>();
+    scan_row<T, W>(xr, begin, end, W > 1 ? wave : 0, top, a, best, &best_floor);
+    a.join();
     if (W > 1) {
-      if (lane == 0) sums[wave] = {a.r, a.s, a.t, best.size};
-      if (lane < top) lists[wave * top + lane] = {lane < best.size ? best.key : kNone, best.cls};
+      if (lane == 0) sums[wave] = {a.r, a.s, a.t};
+      if (wave > 0 && lane < top) lists[wave * top + lane] = {best.val, best.cls};
       __syncthreads();
       if (wave == 0) {
         a = Sums();
@@ -387,34 +474,23 @@ __global__ void __launch_bounds__(kThreads) k_fwd_wide(const T* __restrict__ x, 
           a.s = sums[lane].s;
           a.t = sums[lane].t;
         }
-        a.join<W>();
+        a.join();
+        if (top) {
+          for (int w = 1; w < W; ++w) {
+            Entry e = {__builtin_nanf(""), 0};
+            if (lane < top) e = lists[w * top + lane];
+            best.join(e.val, e.cls, top);
+          }
+        }
       }
     }
     if (W == 1 || wave == 0) {
       if (SPLIT) {
-        if (lane == 0) part[job] = {a.r, a.s, a.t, 0};
-      } else if (lane == 0) {
-        write_row(o, row, xr, classes, a.r, a.s, a.t);
-      }
-      if (top) {
-        const float r = __shfl(a.r, 0), s = __shfl(a.s, 0);
-        const float ls = s == 0.f ? -kInf : logf(s);
-        auto put = [&](int j, int k, int c) {
-          if (lane == 0) {
-            if (SPLIT) {
-              part_top[job * top + j] = {k, c};
-            } else {
-              o.top_class[row * top + j] = c;
-              o.top_logp[row * top + j] = logp_of(value_of(k), r, ls);
-            }
-          }
-        };
-        if (W > 1) {
-          top_of_lists(lists, W * top, top, put);
-        } else if (lane < top) {
-          o.top_class[row * top + lane] = best.cls;
-          o.top_logp[row * top + lane] = logp_of(value_of(best.key), r, ls);
-        }
+        if (lane == 0) part[job] = {a.r, a.s, a.t};
+        if (lane < top) part_top[job * top + lane] = {best.val, best.cls};
+      } else {
+        if (lane == 0) write_row(o, row, xr, classes, a.r, a.s, a.t);
+        write_top(o, row, top, best, a.r, a.s);
       }
     }
     if (W > 1) __syncthreads();  // the next row writes the lists
@@ -426,7 +502,7 @@ template <typename T>
 __global__ void __launch_bounds__(kWave) k_fwd_join(const T* __restrict__ x, int64_t rows,
                                                     int classes, int64_t stride, int top,
                                                     int splits, const Partial* __restrict__ part,
-                                                    const int2* __restrict__ part_top, RowOut o) {
+                                                    const Entry* __restrict__ part_top, RowOut o) {
   const int lane = threadIdx.x;
   for (int64_t row = blockIdx.x; row < rows; row += gridDim.x) {
     Sums a;
@@ -441,16 +517,30 @@ __global__ void __launch_bounds__(kWave) k_fwd_join(const T* __restrict__ x, int
       a.s += b.s;
       a.t += b.t;
     }
-    a.join<64>();
+    a.join();
     if (lane == 0) write_row(o, row, x + row * stride, classes, a.r, a.s, a.t);
-    const float ls = a.s == 0.f ? -kInf : logf(a.s);
-    if (top)
-      top_of_lists(part_top + row * splits * top, splits * top, top, [&](int j, int k, int c) {
-        if (lane == 0) {
-          o.top_class[row * top + j] = c;
-          o.top_logp[row * top + j] = logp_of(value_of(k), a.r, ls);
+    if (top) {
+      Top best;
+      const int n = splits * top;
+      const Entry* from = part_top + row * n;
+      for (int i0 = 0; i0 < n; i0 += 512) {
+        Entry e[8];
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {
+          e[k] = {__builtin_nanf(""), 0};
+          if (i0 + k * 64 + lane < n) e[k] = from[i0 + k * 64 + lane];
         }
-      });
+#pragma unroll 1
+        for (int k = 0; k < 8 && i0 + k * 64 < n; ++k) {
+          Entry c = e[0];
+#pragma unroll
+          for (int i = 1; i < 8; ++i)
+            if (i == k) c = e[i];
+          best.join(c.val, c.cls, top);
+        }
+      }
+      write_top(o, row, top, best, a.r, a.s);
+    }
   }
 }
 
@@ -518,29 +608,17 @@ __device__ __forceinline__ float bwd_dense(const BwdRow& w, float x) {
   return -p * (w.total + w.bonus * (max_f(lp, -1000.f) + w.ent));
 }
 
-template <typename T, int V, bool NARROW>
+// L lanes of a block a row, or a part of one; V elements an access (1: one element)
+template <typename T, int V, int L>
 __global__ void __launch_bounds__(kThreads) k_bwd(const T* __restrict__ x, int64_t rows,
                                                   int classes, int64_t stride, int parts,
                                                   int per_part, BwdArgs b, T* __restrict__ out) {
-  if (NARROW) {
-    // one logit a thread, in the output's order
-    const int64_t n = rows * classes;
-    for (int64_t e = int64_t(blockIdx.x) * kThreads + threadIdx.x; e < n;
-         e += int64_t(gridDim.x) * kThreads) {
-      const int64_t row = e / classes;
-      const int c = int(e - row * classes);
-      const BwdRow w = bwd_row(b, row, classes);
-      float g = w.empty ? 0.f : bwd_dense(w, to_f32(x[row * stride + c]));
-      if (!w.empty && c == w.target) g += w.given;
-      if (b.g_top && !w.empty)
-        for (int j = 0; j < b.top; ++j)
-          if (b.top_class[row * b.top + j] == c) g += b.g_top[row * b.top + j];
-      out[e] = from_f32<T>(g);
-    }
-    return;
-  }
-  for (int64_t job = blockIdx.x; job < rows * parts; job += gridDim.x) {
-    const int64_t row = job / parts;
+  const int lane = threadIdx.x % L;
+  // (known to be uniform, a row's numbers come by scalar loads: 350 -> 320 us over 417M logits)
+  const int team = L >= kThreads ? 0 : L >= kWave ? wave_uniform(threadIdx.x / L) : threadIdx.x / L;
+  const int64_t jobs = rows * parts, step = int64_t(gridDim.x) * (kThreads / L);
+  for (int64_t job = int64_t(blockIdx.x) * (kThreads / L) + team; job < jobs; job += step) {
+    const int64_t row = parts == 1 ? job : job / parts;
     const int begin = int(job - row * parts) * per_part;
     const int end = begin + per_part < classes ? begin + per_part : classes;
     const BwdRow w = bwd_row(b, row, classes);
@@ -563,7 +641,7 @@ __global__ void __launch_bounds__(kThreads) k_bwd(const T* __restrict__ x, int64
       vecs = (end - lo) / V;
       const auto* px = reinterpret_cast<const Pack<T, V>*>(xr + lo);
       auto* pg = reinterpret_cast<Pack<T, V>*>(gr + lo);
-      for (int v = threadIdx.x; v < vecs; v += kThreads) {
+      for (int v = lane; v < vecs; v += L) {
         const Pack<T, V> q = px[v];
         const int c0 = lo + v * V;
         float g[V];
@@ -590,8 +668,9 @@ __global__ void __launch_bounds__(kThreads) k_bwd(const T* __restrict__ x, int64
         pg[v] = r;
       }
     }
-    for (int c = begin + threadIdx.x; c < lo; c += kThreads) at(c);
-    for (int c = lo + vecs * V + threadIdx.x; c < end; c += kThreads) at(c);
+    // what the vectors leave, or everything
+    const int before = lo - begin, tail = lo + vecs * V;
+    for (int i = lane; i < before + end - tail; i += L) at(i < before ? begin + i : tail + i - before);
   }
 }
 
@@ -611,7 +690,7 @@ size_t gfd_class_logp_workspace_size(int64_t rows, int64_t classes, int top) {
   if (s == 1) return 0;
   Sizer z;
   z.take<Partial>(size_t(rows) * s);
-  z.take<int2>(size_t(rows) * s * top);
+  z.take<Entry>(size_t(rows) * s * top);
   return z.off;
 }
 
@@ -630,11 +709,11 @@ gfd_status gfd_class_logp_fwd(const void* logits, int dtype, int64_t rows, int64
   const int n = int(classes);
   const int splits = splits_of(rows, classes);
   Partial* part = nullptr;
-  int2* part_top = nullptr;
+  Entry* part_top = nullptr;
   if (splits > 1) {
     Carve c(ws, ws_bytes);
     part = c.take<Partial>(size_t(rows) * splits);
-    part_top = c.take<int2>(size_t(rows) * splits * top);
+    part_top = c.take<Entry>(size_t(rows) * splits * top);
     if (!c.ok) return GFD_ERR_WORKSPACE;
   }
   return with_dtype(dtype, [&](auto tag) {
@@ -695,21 +774,31 @@ gfd_status gfd_class_logp_bwd(const void* logits, int dtype, int64_t rows, int64
     constexpr int V = 16 / sizeof(T);
     const T* x = static_cast<const T*>(logits);
     T* g = static_cast<T*>(grad_logits);
-    if (n < 512) {
-      const int64_t blocks = (rows * n + kThreads - 1) / kThreads;
-      k_bwd<T, 1, true><<<int(blocks < 65536 ? blocks : 65536), kThreads, 0, stream>>>(
-          x, rows, n, row_stride, 1, n, b, g);
+    auto launch = [&](auto v, auto l, int parts, int per) {
+      constexpr int VV = decltype(v)::value, L = decltype(l)::value;
+      const int64_t blocks = (rows * parts + kThreads / L - 1) / (kThreads / L);
+      k_bwd<T, VV, L><<<int(blocks < 65536 ? blocks : 65536), kThreads, 0, stream>>>(
+          x, rows, n, row_stride, parts, per, b, g);
+    };
+    using std::integral_constant;
+    const integral_constant<int, 1> one;
+    const integral_constant<int, V> vec;
+    // 16-byte vectors where every row of both starts at the same place of one
+    const bool same = (reinterpret_cast<uintptr_t>(x) - reinterpret_cast<uintptr_t>(g)) % 16 == 0 &&
+                      (rows == 1 || (row_stride - classes) * int64_t(sizeof(T)) % 16 == 0);
+    if (n <= 4) {
+      launch(one, integral_constant<int, 1>{}, 1, n);
+    } else if (n <= 16) {
+      launch(one, integral_constant<int, 4>{}, 1, n);
+    } else if (n <= 128) {
+      launch(one, integral_constant<int, 16>{}, 1, n);
+    } else if (n <= kWaveRow) {
+      if (same) launch(vec, integral_constant<int, 64>{}, 1, n);
+      else launch(one, integral_constant<int, 64>{}, 1, n);
     } else {
       const int parts = (n + 8191) / 8192, per = int(align_up(size_t((n + parts - 1) / parts), 16));
-      const int64_t jobs = rows * parts;
-      const int grid = int(jobs < 65536 ? jobs : 65536);
-      // 16-byte vectors where every row of both starts at the same place of one
-      const bool same = (reinterpret_cast<uintptr_t>(x) - reinterpret_cast<uintptr_t>(g)) % 16 == 0 &&
-                        (rows == 1 || (row_stride - classes) * int64_t(sizeof(T)) % 16 == 0);
-      if (same)
-        k_bwd<T, V, false><<<grid, kThreads, 0, stream>>>(x, rows, n, row_stride, parts, per, b, g);
-      else
-        k_bwd<T, 1, false><<<grid, kThreads, 0, stream>>>(x, rows, n, row_stride, parts, per, b, g);
+      if (same) launch(vec, integral_constant<int, 256>{}, parts, per);
+      else launch(one, integral_constant<int, 256>{}, parts, per);
     }
     GFD_LAUNCH_CHECK();
     return GFD_OK;
