@@ -40,8 +40,10 @@ struct Norm {
   double* stats;   // [segments, groups, 2]
   double2* part;   // column sums
   double2* mom;    // backward: A, B of a segment and group
+  void* dw;        // backward, nullable
+  void* db;
   double eps;
-  int channels, groups, w_f32, act;
+  int channels, groups, w_f32;
   int tile;        // rows of a tile; ragged segments up to it are short
   int tiles;       // of one segment (dense) or of all rows (ragged)
   int part0;       // first row of ``part`` that the teams write (backward)
@@ -68,13 +70,17 @@ __device__ __forceinline__ void segment_rows(const Norm& n, int64_t s, int64_t& 
   }
 }
 
-// the last segment that starts at or before row r, -1: none
+// the last segment that starts at or before row r, -1: none.  A whole wave: 64 probes at a time
 __device__ __forceinline__ int64_t segment_of(const Norm& n, int64_t r) {
-  int64_t lo = -1, hi = n.segments;
+  const int lane = threadIdx.x & 63;
+  int64_t lo = -1, hi = n.segments;  // lo starts at or before r, hi does not
   while (hi - lo > 1) {
-    const int64_t mid = (lo + hi) / 2;
-    if (ptr_at(n, mid) <= r) lo = mid;
-    else hi = mid;
+    const int64_t step = (hi - lo - 1 + 63) / 64;
+    const int64_t at = lo + 1 + lane * step;
+    const int before = __popcll(__ballot(at < hi && ptr_at(n, at) <= r));  // the first ones
+    const int64_t base = lo + 1;
+    if (before > 0) lo = base + (before - 1) * step;
+    if (base + before * step < hi) hi = base + before * step;
   }
   return lo;
 }
@@ -92,23 +98,27 @@ __device__ __forceinline__ int pieces_of(const Norm& n, int64_t t, Piece (&p)[2]
     return 1;
   }
   const int64_t a = t * n.tile, e = a + n.tile < n.length ? a + n.tile : n.length;
-  const int64_t s0 = segment_of(n, a), s1 = segment_of(n, e - 1);
   int found = 0;
-#pragma unroll
-  for (int i = 0; i < 2; ++i) {
-    const int64_t s = i == 0 ? s0 : s1;
-    p[i] = {-1, 0, 0};
-    if (s < 0 || (i == 1 && s1 == s0)) continue;
+  auto piece = [&](int i, int64_t s) {
     int64_t r0, r1;
     segment_rows(n, s, r0, r1);
-    if (r1 - r0 <= n.tile) continue;
-    r0 = r0 < a ? a : r0;
-    r1 = r1 > e ? e : r1;
-    if (r0 < r1) {
-      p[i] = {s, r0, r1};
-      found = i + 1;
+    const int64_t to = r1;
+    p[i] = {-1, 0, 0};
+    if (r1 - r0 > n.tile) {
+      r0 = r0 < a ? a : r0;
+      r1 = r1 > e ? e : r1;
+      if (r0 < r1) {
+        p[i] = {s, r0, r1};
+        found = i + 1;
+      }
     }
-  }
+    return to;
+  };
+  const int64_t s0 = segment_of(n, a);
+  p[0] = p[1] = {-1, 0, 0};
+  if (s0 >= 0 && piece(0, s0) >= e) return found;
+  const int64_t s1 = segment_of(n, e - 1);
+  if (s1 >= 0 && s1 != s0) piece(1, s1);
   return found;
 }
 
@@ -128,20 +138,46 @@ __device__ __forceinline__ float affine_at(const void* p, int f32, int c, float 
   return f32 ? static_cast<const float*>(p)[c] : to_f32(static_cast<const T*>(p)[c]);
 }
 
-// activation and, where D is not null, its derivative at z
-__device__ __forceinline__ float activate(float z, int act, float* d) {
-  switch (act) {
+// V of them
+template <typename T, int V>
+__device__ __forceinline__ void affine(const void* p, int f32, int c, float none, float (&v)[V]) {
+#pragma unroll
+  for (int j = 0; j < V; ++j) v[j] = none;
+  if (p && f32) {
+#pragma unroll
+    for (int j = 0; j < V; ++j) v[j] = static_cast<const float*>(p)[c + j];
+  } else if (p) {
+#pragma unroll
+    for (int j = 0; j < V; ++j) v[j] = to_f32(static_cast<const T*>(p)[c + j]);
+  }
+}
+
+__device__ __forceinline__ float exp_of(float v) { return __builtin_amdgcn_exp2f(v * 1.4426950408889634f); }
+
+// activation and, where d is not null, its derivative at z
+template <int ACT>
+__device__ __forceinline__ float activate(float z, float* d) {
+  switch (ACT) {
     case GFD_ACT_RELU:
       if (d) *d = z > 0.f ? 1.f : 0.f;
       return z > 0.f ? z : z != z ? z : 0.f;
     case GFD_ACT_SILU: {
-      const float p = 1.f / (1.f + __expf(-z));
+      const float p = __builtin_amdgcn_rcpf(1.f + exp_of(-z));
       if (d) *d = p * (1.f + z * (1.f - p));
       return z * p;
     }
     case GFD_ACT_GELU: {
-      const float p = 0.5f * (1.f + erff(z * 0.70710678118654752f));
-      if (d) *d = p + z * __expf(-0.5f * z * z) * 0.39894228040143268f;
+      // Phi(z) = (1 + erf(z / sqrt 2)) / 2 with Abramowitz and Stegun's 7.1.26: the tail
+      // e^(-z^2 / 2) times a polynomial in 1 / (1 + p |z| / sqrt 2), within 7.5e-8; its
+      // exponential is the derivative's too
+      const float e = exp_of(-0.5f * z * z);
+      const float t = __builtin_amdgcn_rcpf(fmaf(fabsf(z), 0.3275911f * 0.70710678118654752f, 1.f));
+      float q = fmaf(t, 0.5f * 1.061405429f, 0.5f * -1.453152027f);
+      q = fmaf(t, q, 0.5f * 1.421413741f);
+      q = fmaf(t, q, 0.5f * -0.284496736f);
+      q = fmaf(t, q, 0.5f * 0.254829592f) * t * e;
+      const float p = z > 0.f ? 1.f - q : q;
+      if (d) *d = fmaf(z * e, 0.39894228040143268f, p);
       return z * p;
     }
     default:
@@ -150,72 +186,68 @@ __device__ __forceinline__ float activate(float z, int act, float* d) {
   }
 }
 
-struct Moments {
+// The columns of one vector in one segment: z = d A + B and xhat = d r - lr with d = x - hi, the
+// mean split into hi + lo so that nothing is lost where it is far larger than the spread
+template <typename T, int V, int ACT>
+struct Columns {
   double mean, rstd;
-  float hi, lo, r;  // mean = hi + lo
-  __device__ __forceinline__ Moments(double m, double s) : mean(m), rstd(s) {
-    hi = float(m);
-    lo = float(m - double(hi));
-    r = float(s);
-  }
-  __device__ __forceinline__ float xhat(float x) const { return ((x - hi) - lo) * r; }
-  // xhat w + b; where it is too near 0 for fp32 to tell relu's side, from fp64
-  __device__ __forceinline__ float z(float x, float xh, float w, float b, int act) const {
-    const float p = xh * w, v = p + b;
-    if (act == GFD_ACT_RELU && fabsf(v) <= 1e-5f * (fabsf(p) + fabsf(b)))
-      return float((double(x) - mean) * rstd * double(w) + double(b));
-    return v;
-  }
-};
+  float hi, r, lr;
+  float A[V], B[V];
+  int c0;
 
-template <typename T, int V>
-struct Affine {
-  float w[V], b[V];
-  __device__ __forceinline__ void load(const Norm& n, int col) {
+  __device__ __forceinline__ void set(const Norm& n, int col, double m, double s) {
+    mean = m;
+    rstd = s;
+    hi = float(m);
+    r = float(s);
+    lr = float((m - double(hi)) * s);
+    c0 = col * V;
+    affine<T, V>(n.w, n.w_f32, c0, 1.f, A);
+    affine<T, V>(n.b, n.w_f32, c0, 0.f, B);
 #pragma unroll
     for (int j = 0; j < V; ++j) {
-      w[j] = affine_at<T>(n.w, n.w_f32, col * V + j, 1.f);
-      b[j] = affine_at<T>(n.b, n.w_f32, col * V + j, 0.f);
+      B[j] = fmaf(-lr, A[j], B[j]);
+      A[j] *= r;
     }
   }
+  // z; where it is too near 0 for fp32 to tell relu's side, from fp64
+  __device__ __forceinline__ float z(const Norm& n, float x, float d, int j) const {
+    const float v = fmaf(d, A[j], B[j]);
+    if (ACT == GFD_ACT_RELU && fabsf(v) <= 2e-6f * (fabsf(d * A[j]) + fabsf(B[j])))
+      return float((double(x) - mean) * rstd * double(affine_at<T>(n.w, n.w_f32, c0 + j, 1.f)) +
+                   double(affine_at<T>(n.b, n.w_f32, c0 + j, 0.f)));
+    return v;
+  }
+  __device__ __forceinline__ Pack<T, V> forward(const Norm& n, const Raw<T, V>& x) const {
+    Pack<T, V> y;
+#pragma unroll
+    for (int j = 0; j < V; ++j) {
+      const float v = x.at(j);
+      y.v[j] = from_f32<T>(activate<ACT>(z(n, v, v - hi, j), nullptr));
+    }
+    return y;
+  }
+  // dz and xhat
+  __device__ __forceinline__ void slope(const Norm& n, const Raw<T, V>& x, const Raw<T, V>& dy,
+                                        float (&dz)[V], float (&xh)[V]) const {
+#pragma unroll
+    for (int j = 0; j < V; ++j) {
+      const float v = x.at(j), d = v - hi;
+      xh[j] = fmaf(d, r, -lr);
+      float g;
+      activate<ACT>(z(n, v, d, j), &g);
+      dz[j] = dy.at(j) * g;
+    }
+  }
+  // ra, rb: r times the means of w dz and of w dz xhat
+  __device__ __forceinline__ Pack<T, V> backward(const float (&dz)[V], const float (&xh)[V], float ra,
+                                                 float rb) const {
+    Pack<T, V> g;
+#pragma unroll
+    for (int j = 0; j < V; ++j) g.v[j] = from_f32<T>(fmaf(-xh[j], rb, fmaf(A[j], dz[j], -ra)));
+    return g;
+  }
 };
-
-template <typename T, int V>
-__device__ __forceinline__ Pack<T, V> forward(const Pack<T, V>& x, const Moments& m,
-                                              const Affine<T, V>& a, int act) {
-  Pack<T, V> y;
-#pragma unroll
-  for (int j = 0; j < V; ++j) {
-    const float v = to_f32(x.v[j]), xh = m.xhat(v);
-    y.v[j] = from_f32<T>(activate(m.z(v, xh, a.w[j], a.b[j], act), act, nullptr));
-  }
-  return y;
-}
-
-// dz and xhat of one vector
-template <typename T, int V>
-__device__ __forceinline__ void slope(const Pack<T, V>& x, const Pack<T, V>& dy, const Moments& m,
-                                      const Affine<T, V>& a, int act, float (&dz)[V],
-                                      float (&xh)[V]) {
-#pragma unroll
-  for (int j = 0; j < V; ++j) {
-    const float v = to_f32(x.v[j]);
-    xh[j] = m.xhat(v);
-    float d;
-    activate(m.z(v, xh[j], a.w[j], a.b[j], act), act, &d);
-    dz[j] = to_f32(dy.v[j]) * d;
-  }
-}
-
-template <typename T, int V>
-__device__ __forceinline__ Pack<T, V> backward(const float (&dz)[V], const float (&xh)[V],
-                                               const Moments& m, const Affine<T, V>& a, float ma,
-                                               float mb) {
-  Pack<T, V> g;
-#pragma unroll
-  for (int j = 0; j < V; ++j) g.v[j] = from_f32<T>(m.r * (a.w[j] * dz[j] - ma - xh[j] * mb));
-  return g;
-}
 
 // mean and 1 / sqrt(var + eps) from the sums of x and x^2 over n elements
 __device__ __forceinline__ double2 moments_of(double s, double q, double n, double eps) {
@@ -225,130 +257,175 @@ __device__ __forceinline__ double2 moments_of(double s, double q, double n, doub
   return {mean, 1.0 / sqrt(var + eps)};
 }
 
+// the sum over the threads of a block that share a column (threadIdx.x % cols), in those of the
+// first row: lanes of a wave by exchange, waves through LDS; a fixed order
+__device__ __forceinline__ double2 sum_rows(double2 v, int cols, double2* red) {
+  for (int d = cols; d < kWave; d <<= 1) {
+    v.x += __shfl_xor(v.x, d);
+    v.y += __shfl_xor(v.y, d);
+  }
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int step = cols < kWave ? 1 : cols / kWave, width = cols < kWave ? cols : kWave;
+  if (step * kWave < int(blockDim.x)) {
+    __syncthreads();  // the last sum has been read
+    if (lane < width) red[threadIdx.x] = v;
+    __syncthreads();
+    if (wave < step)
+      for (int w = wave + step; w < int(blockDim.x) / kWave; w += step) {
+        v.x += red[w * kWave + lane % width].x;
+        v.y += red[w * kWave + lane % width].y;
+      }
+  }
+  return v;
+}
+
 // ---------------------------------------------------------------------------
 // short segments: a team of cols x rows threads each
 // ---------------------------------------------------------------------------
-template <typename T, int V, int NC, bool BWD>
+template <typename T, int V, int NC, bool BWD, int ACT>
 __global__ void __launch_bounds__(kMaxTeam) k_team(const Norm n) {
   extern __shared__ double2 lds[];
-  double2* red = lds;                 // [blockDim]
+  double2* red = lds;                   // [blockDim]
   double2* col_sum = lds + blockDim.x;  // [teams][vecs]
   using P = Pack<T, V>;
   const int vecs = n.channels / V, gv = vecs / n.groups;
   const int size = n.cols * n.rows, teams = blockDim.x / size;
   const int c = threadIdx.x % n.cols, tr = threadIdx.x / n.cols % n.rows, team = threadIdx.x / size;
-  Affine<T, V> aff[NC];
   double dw[NC][V] = {}, db[NC][V] = {};
-#pragma unroll
-  for (int k = 0; k < NC; ++k)
-    if (c + k * n.cols < vecs) aff[k].load(n, c + k * n.cols);
   for (int64_t s0 = int64_t(blockIdx.x) * teams; s0 < n.segments; s0 += int64_t(gridDim.x) * teams) {
+    auto rows_of = [&](int64_t s, int64_t& r0, int64_t& r1) {
+      r0 = r1 = 0;
+      if (s < n.segments) {
+        segment_rows(n, s, r0, r1);
+        if (n.ptr && r1 - r0 > n.tile) r1 = r0;  // a long one: not here
+      }
+    };
     const int64_t seg = s0 + team;
-    int64_t r0 = 0, r1 = 0;
-    if (seg < n.segments) {
-      segment_rows(n, seg, r0, r1);
-      if (n.ptr && r1 - r0 > n.tile) r1 = r0;  // a long one: not here
-    }
-    // sums of each column: x and x^2, or w dz and w dz xhat
+    int64_t r0, r1;
+    rows_of(seg, r0, r1);
+    const bool any = r0 < r1;
+    auto x_at = [&](int64_t r, int col) {
+      Raw<T, V> v;
+      v.read(row_in<T>(n, n.x, seg, r) + col * V);
+      return v;
+    };
+    auto dy_at = [&](int64_t r, int col) {
+      Raw<T, V> v;
+      v.read(static_cast<const T*>(n.dy) + r * n.channels + col * V);
+      return v;
+    };
+    // sums over the rows by column (f(k, col, a, b) adds a thread's), then of each group, handed
+    // to done(segment, group, a, b, its number of elements) and left at its first column
+    auto reduce = [&](auto f, auto done) {
 #pragma unroll
-    for (int k = 0; k < NC; ++k) {
-      const int col = c + k * n.cols;
-      double a = 0.0, b = 0.0;
-      if (col < vecs && r0 < r1) {
-        double mean = 0.0, rstd = 0.0;
-        if (BWD) {
-          const double* st = n.stats + 2 * (seg * n.groups + col / gv);
-          mean = st[0];
-          rstd = st[1];
-        }
-        const Moments m(mean, rstd);
-        for (int64_t r = r0 + tr; r < r1; r += n.rows) {
-          const P x = *reinterpret_cast<const P*>(row_in<T>(n, n.x, seg, r) + col * V);
-          if (BWD) {
-            const P dy = *reinterpret_cast<const P*>(static_cast<const T*>(n.dy) + r * n.channels + col * V);
-            float dz[V], xh[V];
-            slope<T, V>(x, dy, m, aff[k], n.act, dz, xh);
-#pragma unroll
-            for (int j = 0; j < V; ++j) {
-              const double e = double(dz[j]), f = e * double(xh[j]);
-              db[k][j] += e;
-              dw[k][j] += f;
-              a += double(aff[k].w[j]) * e;
-              b += double(aff[k].w[j]) * f;
+      for (int k = 0; k < NC; ++k) {
+        const int col = c + k * n.cols;
+        double a = 0.0, b = 0.0;
+        if (col < vecs && any) f(k, col, a, b);
+        if (n.rows > 1) {
+          red[threadIdx.x] = {a, b};
+          __syncthreads();
+          if (tr == 0)
+            for (int i = 1; i < n.rows; ++i) {
+              a += red[threadIdx.x + i * n.cols].x;
+              b += red[threadIdx.x + i * n.cols].y;
             }
-          } else {
-#pragma unroll
-            for (int j = 0; j < V; ++j) {
-              const double v = double(to_f32(x.v[j]));
-              a += v;
-              b += v * v;
-            }
-          }
         }
-      }
-      if (n.rows > 1) {
-        red[threadIdx.x] = {a, b};
+        if (tr == 0 && col < vecs) col_sum[team * vecs + col] = {a, b};
         __syncthreads();
-        if (tr == 0)
-          for (int i = 1; i < n.rows; ++i) {
-            a += red[threadIdx.x + i * n.cols].x;
-            b += red[threadIdx.x + i * n.cols].y;
-          }
       }
-      if (tr == 0 && col < vecs) col_sum[team * vecs + col] = {a, b};
-      __syncthreads();
-    }
-    // of each group, in place of its first column
-    for (int i = threadIdx.x; i < teams * n.groups; i += blockDim.x) {
-      const int tm = i / n.groups, g = i - tm * n.groups;
-      const int64_t sg = s0 + tm;
-      int64_t q0 = 0, q1 = 0;
-      if (sg < n.segments) {
-        segment_rows(n, sg, q0, q1);
-        if (n.ptr && q1 - q0 > n.tile) q1 = q0;
-      }
-      if (q0 >= q1) continue;
-      double2* cs = col_sum + tm * vecs + g * gv;
-      double a = 0.0, b = 0.0;
-      for (int k = 0; k < gv; ++k) {
-        a += cs[k].x;
-        b += cs[k].y;
-      }
-      const double count = double(q1 - q0) * (n.channels / n.groups);
-      if (BWD) {
-        cs[0] = {a / count, b / count};
-      } else {
-        const double2 m = moments_of(a, b, count, n.eps);
-        cs[0] = m;
-        if (n.stats) {
-          n.stats[2 * (sg * n.groups + g)] = m.x;
-          n.stats[2 * (sg * n.groups + g) + 1] = m.y;
+      for (int i = threadIdx.x; i < teams * n.groups; i += blockDim.x) {
+        const int tm = i / n.groups, g = i - tm * n.groups;
+        int64_t q0, q1;
+        rows_of(s0 + tm, q0, q1);
+        if (q0 >= q1) continue;
+        double2* cs = col_sum + tm * vecs + g * gv;
+        double a = 0.0, b = 0.0;
+        for (int k = 0; k < gv; ++k) {
+          a += cs[k].x;
+          b += cs[k].y;
         }
+        cs[0] = done(s0 + tm, g, a, b, double(q1 - q0) * (n.channels / n.groups));
       }
-    }
-    __syncthreads();
+      __syncthreads();
+    };
+    Columns<T, V, ACT> cols[NC];
+    float ra[NC] = {}, rb[NC] = {};
+    const bool kept = BWD && n.stats;  // the forward's moments; else they are found (again)
+    if (!kept)
+      reduce(
+          [&](int, int col, double& a, double& b) {
+            for (int64_t r = r0 + tr; r < r1; r += n.rows) {
+              const Raw<T, V> x = x_at(r, col);
+#pragma unroll
+              for (int j = 0; j < V; ++j) {
+                const double v = double(x.at(j));
+                a += v;
+                b += v * v;
+              }
+            }
+          },
+          [&](int64_t s, int g, double a, double b, double count) {
+            const double2 m = moments_of(a, b, count, n.eps);
+            if (!BWD && n.stats) {
+              n.stats[2 * (s * n.groups + g)] = m.x;
+              n.stats[2 * (s * n.groups + g) + 1] = m.y;
+            }
+            return m;
+          });
 #pragma unroll
     for (int k = 0; k < NC; ++k) {
       const int col = c + k * n.cols;
-      if (col < vecs && r0 < r1) {
-        const double2 v = col_sum[team * vecs + col / gv * gv];
-        double mean = v.x, rstd = v.y;
-        if (BWD) {
+      if (col < vecs && any) {
+        if (kept) {
           const double* st = n.stats + 2 * (seg * n.groups + col / gv);
-          mean = st[0];
-          rstd = st[1];
+          cols[k].set(n, col, st[0], st[1]);
+        } else {
+          const double2 m = col_sum[team * vecs + col / gv * gv];
+          cols[k].set(n, col, m.x, m.y);
         }
-        const Moments m(mean, rstd);
+      }
+    }
+    if (BWD) {
+      if (!kept) __syncthreads();
+      reduce(
+          [&](int k, int col, double& a, double& b) {
+            for (int64_t r = r0 + tr; r < r1; r += n.rows) {
+              float dz[V], xh[V];
+              cols[k].slope(n, x_at(r, col), dy_at(r, col), dz, xh);
+#pragma unroll
+              for (int j = 0; j < V; ++j) {
+                const double e = double(dz[j]), f = double(dz[j] * xh[j]);
+                db[k][j] += e;
+                dw[k][j] += f;
+                a += double(cols[k].A[j]) * e;  // r times w
+                b += double(cols[k].A[j]) * f;
+              }
+            }
+          },
+          [&](int64_t, int, double a, double b, double count) { return double2{a / count, b / count}; });
+#pragma unroll
+      for (int k = 0; k < NC; ++k) {
+        const int col = c + k * n.cols;
+        if (col < vecs && any) {
+          const double2 v = col_sum[team * vecs + col / gv * gv];
+          ra[k] = float(v.x);
+          rb[k] = float(v.y);
+        }
+      }
+    }
+#pragma unroll
+    for (int k = 0; k < NC; ++k) {
+      const int col = c + k * n.cols;
+      if (col < vecs && any) {
         for (int64_t r = r0 + tr; r < r1; r += n.rows) {
-          const P x = *reinterpret_cast<const P*>(row_in<T>(n, n.x, seg, r) + col * V);
           P* out = reinterpret_cast<P*>(static_cast<T*>(n.out) + r * n.channels + col * V);
           if (BWD) {
-            const P dy = *reinterpret_cast<const P*>(static_cast<const T*>(n.dy) + r * n.channels + col * V);
             float dz[V], xh[V];
-            slope<T, V>(x, dy, m, aff[k], n.act, dz, xh);
-            *out = backward<T, V>(dz, xh, m, aff[k], float(v.x), float(v.y));
+            cols[k].slope(n, x_at(r, col), dy_at(r, col), dz, xh);
+            *out = cols[k].backward(dz, xh, ra[k], rb[k]);
           } else {
-            *out = forward<T, V>(x, m, aff[k], n.act);
+            *out = cols[k].forward(n, x_at(r, col));
           }
         }
       }
@@ -362,17 +439,8 @@ __global__ void __launch_bounds__(kMaxTeam) k_team(const Norm n) {
       const int col = c + k * n.cols;
 #pragma unroll
       for (int j = 0; j < V; ++j) {
-        red[threadIdx.x] = {db[k][j], dw[k][j]};
-        __syncthreads();
-        if (threadIdx.x < n.cols && col < vecs) {
-          double2 t = red[threadIdx.x];
-          for (int i = threadIdx.x + n.cols; i < int(blockDim.x); i += n.cols) {
-            t.x += red[i].x;
-            t.y += red[i].y;
-          }
-          part[col * V + j] = t;
-        }
-        __syncthreads();
+        const double2 v = sum_rows({db[k][j], dw[k][j]}, n.cols, red);
+        if (threadIdx.x < n.cols && col < vecs) part[col * V + j] = v;
       }
     }
   }
@@ -385,154 +453,213 @@ constexpr int kTileThreads = 256;
 
 // column sums of a tile: forward [slot][vecs] of x and x^2, backward [slot][channels] of dz and
 // dz xhat; ragged tiles have two slots, an unused one is 0
-template <typename T, int V, bool BWD>
+template <typename T, int V, bool BWD, int ACT>
 __global__ void __launch_bounds__(kTileThreads) k_sums(const Norm n) {
-  using P = Pack<T, V>;
   constexpr int S = BWD ? V : 1;
+  constexpr int R = BWD ? 4 : 8;  // rows in flight
   __shared__ double2 red[kTileThreads];
   const int vecs = n.channels / V, gv = vecs / n.groups;
   const int c = threadIdx.x % n.cols, tr = threadIdx.x / n.cols, rows = kTileThreads / n.cols;
   const int col = blockIdx.y * n.cols + c;
   const int64_t t = blockIdx.x;
-  Affine<T, V> aff;
-  if (BWD && col < vecs) aff.load(n, col);
   Piece p[2];
   const int found = pieces_of(n, t, p);
+#pragma unroll 1
   for (int i = 0; i < (n.ptr ? 2 : 1); ++i) {
+    const bool here = i < found && p[i].seg >= 0;
     double a[S] = {}, b[S] = {};
-    if (i < found && p[i].seg >= 0 && col < vecs) {
-      double mean = 0.0, rstd = 0.0;
+    if (here && col < vecs) {
+      Columns<T, V, ACT> k;
       if (BWD) {
         const double* st = n.stats + 2 * (p[i].seg * n.groups + col / gv);
-        mean = st[0];
-        rstd = st[1];
+        k.set(n, col, st[0], st[1]);
       }
-      const Moments m(mean, rstd);
-#pragma unroll 4
-      for (int64_t r = p[i].r0 + tr; r < p[i].r1; r += rows) {
-        const P x = *reinterpret_cast<const P*>(row_in<T>(n, n.x, p[i].seg, r) + col * V);
+      const T* px = row_in<T>(n, n.x, p[i].seg, p[i].r0 + tr) + col * V;
+      const T* pd = static_cast<const T*>(n.dy) + (p[i].r0 + tr) * n.channels + col * V;
+      const int64_t xs = rows * n.row_stride, ds = int64_t(rows) * n.channels;
+      int64_t left = p[i].r1 - p[i].r0 - tr;
+      auto take = [&](auto number) {  // that many rows, all of them read first
+        constexpr int N = decltype(number)::value;
+        Raw<T, V> x[N], dy[N];
+#pragma unroll
+        for (int u = 0; u < N; ++u) {
+          x[u].read(px + u * xs);
+          if (BWD) dy[u].read(pd + u * ds);
+        }
+        px += N * xs;
+        pd += N * ds;
+        left -= N * rows;
         if (BWD) {
-          const P dy = *reinterpret_cast<const P*>(static_cast<const T*>(n.dy) + r * n.channels + col * V);
-          float dz[V], xh[V];
-          slope<T, V>(x, dy, m, aff, n.act, dz, xh);
+          float e[V] = {}, f[V] = {};  // of N rows in fp32
+#pragma unroll
+          for (int u = 0; u < N; ++u) {
+            float dz[V], xh[V];
+            k.slope(n, x[u], dy[u], dz, xh);
+#pragma unroll
+            for (int j = 0; j < V; ++j) {
+              e[j] += dz[j];
+              f[j] = fmaf(dz[j], xh[j], f[j]);
+            }
+          }
 #pragma unroll
           for (int j = 0; j < V; ++j) {
-            a[j % S] += double(dz[j]);
-            b[j % S] += double(dz[j]) * double(xh[j]);
+            a[j % S] += double(e[j]);
+            b[j % S] += double(f[j]);
           }
         } else {
 #pragma unroll
-          for (int j = 0; j < V; ++j) {
-            const double v = double(to_f32(x.v[j]));
-            a[0] += v;
-            b[0] += v * v;
-          }
+          for (int u = 0; u < N; ++u)
+#pragma unroll
+            for (int j = 0; j < V; ++j) {
+              const double v = double(x[u].at(j));
+              a[0] += v;
+              b[0] += v * v;
+            }
         }
-      }
+      };
+      while (left > (R - 1) * rows) take(std::integral_constant<int, R>{});
+      while (left > 0) take(std::integral_constant<int, 1>{});
     }
     const int64_t slot = n.ptr ? 2 * t + i : t;
 #pragma unroll
     for (int j = 0; j < S; ++j) {
-      red[threadIdx.x] = {a[j], b[j]};
-      __syncthreads();
-      if (tr == 0 && col < vecs) {
-        double2 v = red[c];
-        for (int k = 1; k < rows; ++k) {
-          v.x += red[c + k * n.cols].x;
-          v.y += red[c + k * n.cols].y;
-        }
-        n.part[slot * (BWD ? n.channels : vecs) + col * S + j] = v;
-      }
-      __syncthreads();
+      double2 v = {a[j], b[j]};
+      if (here) v = sum_rows(v, n.cols, red);
+      if (tr == 0 && col < vecs) n.part[slot * (BWD ? n.channels : vecs) + col * S + j] = v;
     }
   }
 }
 
-__device__ __forceinline__ double wave_sum(double v) {
-#pragma unroll
-  for (int d = 1; d < 64; d <<= 1) v += __shfl_xor(v, d);
-  return v;
+constexpr int kJoinThreads = 256;
+
+// the weight and bias gradients of 4 channels: their column sums of all slots in a fixed order
+template <typename T>
+__device__ void join_columns(const Norm& n, int64_t slots, int c0, double2* red) {
+  const int c = c0 + (threadIdx.x & 3);
+  double2 s = {0.0, 0.0};
+  if (c < n.channels) {
+#pragma unroll 4
+    for (int64_t i = threadIdx.x >> 2; i < slots; i += kJoinThreads / 4) {
+      const double2 v = n.part[i * n.channels + c];
+      s.x += v.x;
+      s.y += v.y;
+    }
+  }
+  s = sum_rows(s, 4, red);
+  if (threadIdx.x < 4 && c < n.channels) {
+    if (n.db) {
+      if (n.w_f32) static_cast<float*>(n.db)[c] = float(s.x);
+      else static_cast<T*>(n.db)[c] = from_f32<T>(float(s.x));
+    }
+    if (n.dw) {
+      if (n.w_f32) static_cast<float*>(n.dw)[c] = float(s.y);
+      else static_cast<T*>(n.dw)[c] = from_f32<T>(float(s.y));
+    }
+  }
 }
 
-// a wave for each long segment and group: its tiles' sums
+// a block for each long segment and group, its tiles' sums (blocks from 0 to jobs); behind them
+// a block for every 4 channels of the weight and bias gradients
 template <typename T, int V, bool BWD>
-__global__ void __launch_bounds__(kWave) k_stats(const Norm n) {
+__global__ void __launch_bounds__(kJoinThreads) k_join(const Norm n, int64_t jobs, int64_t slots) {
+  __shared__ double2 red[kJoinThreads];
+  if (BWD && int64_t(blockIdx.x) >= jobs) {
+    join_columns<T>(n, slots, int(blockIdx.x - jobs) * 4, red);
+    return;
+  }
   const int vecs = n.channels / V, per = n.channels / n.groups;
   const int width = BWD ? n.channels : vecs, each = BWD ? per : vecs / n.groups;
-  for (int64_t job = blockIdx.x; job < n.segments * n.groups; job += gridDim.x) {
-    const int64_t s = job / n.groups;
-    const int g = int(job - s * n.groups);
-    int64_t r0, r1, first, count;
-    segment_rows(n, s, r0, r1);
-    if (n.ptr) {
-      if (r1 - r0 <= n.tile) continue;
-      first = r0 / n.tile;
-      count = (r1 - 1) / n.tile - first + 1;
+  const int64_t job = blockIdx.x, s = job / n.groups;
+  const int g = int(job - s * n.groups);
+  int64_t r0, r1, first, count;
+  segment_rows(n, s, r0, r1);
+  if (n.ptr) {
+    if (r1 - r0 <= n.tile) return;
+    first = r0 / n.tile;
+    count = (r1 - 1) / n.tile - first + 1;
+  } else {
+    first = s * n.tiles;
+    count = n.tiles;
+  }
+  double2 v = {0.0, 0.0};
+#pragma unroll 4
+  for (int64_t i = threadIdx.x; i < count * each; i += kJoinThreads) {
+    const int64_t k = i / each;
+    const int c = int(i - k * each) + g * each;
+    int64_t slot = first + k;
+    // ragged: the second slot where the segment starts inside the tile
+    if (n.ptr) slot = 2 * slot + (r0 > slot * n.tile ? 1 : 0);
+    const double2 q = n.part[slot * width + c];
+    const double w = BWD ? double(affine_at<T>(n.w, n.w_f32, c, 1.f)) : 1.0;
+    v.x += w * q.x;
+    v.y += w * q.y;
+  }
+  v = sum_rows(v, 1, red);
+  if (threadIdx.x == 0) {
+    const double total = double(r1 - r0) * per;
+    if (BWD) {
+      n.mom[job] = {v.x / total, v.y / total};
     } else {
-      first = s * n.tiles;
-      count = n.tiles;
-    }
-    double a = 0.0, b = 0.0;
-    for (int64_t i = threadIdx.x; i < count * each; i += kWave) {
-      const int64_t k = i / each;
-      const int c = int(i - k * each) + g * each;
-      int64_t slot = first + k;
-      // ragged: the second slot where the segment starts inside the tile
-      if (n.ptr) slot = 2 * slot + (r0 > slot * n.tile ? 1 : 0);
-      const double2 v = n.part[slot * width + c];
-      const double w = BWD ? double(affine_at<T>(n.w, n.w_f32, c, 1.f)) : 1.0;
-      a += w * v.x;
-      b += w * v.y;
-    }
-    a = wave_sum(a);
-    b = wave_sum(b);
-    if (threadIdx.x == 0) {
-      const double total = double(r1 - r0) * per;
-      if (BWD) {
-        n.mom[job] = {a / total, b / total};
-      } else {
-        const double2 m = moments_of(a, b, total, n.eps);
-        n.stats[2 * job] = m.x;
-        n.stats[2 * job + 1] = m.y;
-      }
+      const double2 m = moments_of(v.x, v.y, total, n.eps);
+      n.stats[2 * job] = m.x;
+      n.stats[2 * job + 1] = m.y;
     }
   }
 }
 
-template <typename T, int V, bool BWD>
+template <typename T, int V, bool BWD, int ACT>
 __global__ void __launch_bounds__(kTileThreads) k_apply(const Norm n) {
   using P = Pack<T, V>;
   const int vecs = n.channels / V, gv = vecs / n.groups;
   const int c = threadIdx.x % n.cols, tr = threadIdx.x / n.cols, rows = kTileThreads / n.cols;
   const int col = blockIdx.y * n.cols + c;
-  if (col >= vecs) return;
   const int64_t t = blockIdx.x;
-  Affine<T, V> aff;
-  aff.load(n, col);
   Piece p[2];
   const int found = pieces_of(n, t, p);
+  if (col >= vecs) return;
+  constexpr int R = 4;  // rows in flight
   for (int i = 0; i < found; ++i) {
     if (p[i].seg < 0) continue;
     const int64_t job = p[i].seg * n.groups + col / gv;
-    const Moments m(n.stats[2 * job], n.stats[2 * job + 1]);
-    float ma = 0.f, mb = 0.f;
+    Columns<T, V, ACT> k;
+    k.set(n, col, n.stats[2 * job], n.stats[2 * job + 1]);
+    float ra = 0.f, rb = 0.f;
     if (BWD) {
-      ma = float(n.mom[job].x);
-      mb = float(n.mom[job].y);
+      ra = float(n.mom[job].x * k.rstd);
+      rb = float(n.mom[job].y * k.rstd);
     }
-#pragma unroll 4
-    for (int64_t r = p[i].r0 + tr; r < p[i].r1; r += rows) {
-      const P x = *reinterpret_cast<const P*>(row_in<T>(n, n.x, p[i].seg, r) + col * V);
-      P* out = reinterpret_cast<P*>(static_cast<T*>(n.out) + r * n.channels + col * V);
-      if (BWD) {
-        const P dy = *reinterpret_cast<const P*>(static_cast<const T*>(n.dy) + r * n.channels + col * V);
-        float dz[V], xh[V];
-        slope<T, V>(x, dy, m, aff, n.act, dz, xh);
-        *out = backward<T, V>(dz, xh, m, aff, ma, mb);
-      } else {
-        *out = forward<T, V>(x, m, aff, n.act);
+    const T* px = row_in<T>(n, n.x, p[i].seg, p[i].r0 + tr) + col * V;
+    const int64_t at = (p[i].r0 + tr) * n.channels + col * V;
+    const T* pd = static_cast<const T*>(n.dy) + at;
+    T* po = static_cast<T*>(n.out) + at;
+    const int64_t xs = rows * n.row_stride, ds = int64_t(rows) * n.channels;
+    int64_t left = p[i].r1 - p[i].r0 - tr;
+    auto take = [&](auto number) {  // that many rows, all of them read first
+      constexpr int N = decltype(number)::value;
+      Raw<T, V> x[N], dy[N];
+#pragma unroll
+      for (int u = 0; u < N; ++u) {
+        x[u].read(px + u * xs);
+        if (BWD) dy[u].read(pd + u * ds);
       }
-    }
+#pragma unroll
+      for (int u = 0; u < N; ++u) {
+        P* out = reinterpret_cast<P*>(po + u * ds);
+        if (BWD) {
+          float dz[V], xh[V];
+          k.slope(n, x[u], dy[u], dz, xh);
+          *out = k.backward(dz, xh, ra, rb);
+        } else {
+          *out = k.forward(n, x[u]);
+        }
+      }
+      px += N * xs;
+      pd += N * ds;
+      po += N * ds;
+      left -= N * rows;
+    };
+    while (left > (R - 1) * rows) take(std::integral_constant<int, R>{});
+    while (left > 0) take(std::integral_constant<int, 1>{});
   }
   if (n.ptr) {  // the rows of no segment
     const int64_t a = t * n.tile, e = a + n.tile < n.length ? a + n.tile : n.length;
@@ -540,37 +667,6 @@ __global__ void __launch_bounds__(kTileThreads) k_apply(const Norm n) {
     for (int64_t r = a + tr; r < e; r += rows)
       if (r < first || r >= last)
         *reinterpret_cast<P*>(static_cast<T*>(n.out) + r * n.channels + col * V) = P{};
-  }
-}
-
-// the weight and bias gradients: a channel's column sums of all slots in a fixed order
-template <typename T>
-__global__ void __launch_bounds__(256) k_columns(const double2* __restrict__ part, int64_t slots,
-                                                 int channels, int w_f32, void* dw, void* db) {
-  __shared__ double2 red[256];
-  const int c = blockIdx.x * 8 + (threadIdx.x & 7), k = threadIdx.x >> 3;
-  double2 s = {0.0, 0.0};
-  if (c < channels)
-    for (int64_t i = k; i < slots; i += 32) {
-      const double2 v = part[i * channels + c];
-      s.x += v.x;
-      s.y += v.y;
-    }
-  red[threadIdx.x] = s;
-  __syncthreads();
-  if (k == 0 && c < channels) {
-    for (int i = 1; i < 32; ++i) {
-      s.x += red[threadIdx.x + 8 * i].x;
-      s.y += red[threadIdx.x + 8 * i].y;
-    }
-    if (db) {
-      if (w_f32) static_cast<float*>(db)[c] = float(s.x);
-      else static_cast<T*>(db)[c] = from_f32<T>(float(s.x));
-    }
-    if (dw) {
-      if (w_f32) static_cast<float*>(dw)[c] = float(s.y);
-      else static_cast<T*>(dw)[c] = from_f32<T>(float(s.y));
-    }
   }
 }
 
@@ -618,10 +714,11 @@ bool shape_ok(int64_t segments, int64_t length, int channels, int groups) {
          segments <= (int64_t(1) << 40) && length <= (int64_t(1) << 40);
 }
 
-// the widest vector that divides a group's channels and that every row starts at
+// the widest vector, of at most 4, that divides a group's channels and that every row starts at
+// (8 16-bit channels a thread cost more in registers than their wider access brings)
 int vector_of(int64_t per_group, size_t size, const void* const* ptrs, int n, int64_t row_stride,
               int64_t seg_stride) {
-  int v = int(16 / size);
+  int v = 4;
   for (; v > 1; v >>= 1) {
     bool ok = per_group % v == 0 && row_stride % v == 0 && seg_stride % v == 0;
     for (int i = 0; i < n; ++i) ok = ok && aligned_to(ptrs[i], size * v);
@@ -633,17 +730,26 @@ int vector_of(int64_t per_group, size_t size, const void* const* ptrs, int n, in
 template <typename F>
 gfd_status with_vector(int v, F f) {
   switch (v) {
-    case 8: return f(std::integral_constant<int, 8>{});
     case 4: return f(std::integral_constant<int, 4>{});
     case 2: return f(std::integral_constant<int, 2>{});
     default: return f(std::integral_constant<int, 1>{});
   }
 }
 
-template <typename T, int V, bool BWD>
-gfd_status launch(Norm n, const Cut& c, int64_t* team_blocks, hipStream_t stream) {
+template <typename F>
+gfd_status with_act(int act, F f) {
+  switch (act) {
+    case GFD_ACT_RELU: return f(std::integral_constant<int, GFD_ACT_RELU>{});
+    case GFD_ACT_SILU: return f(std::integral_constant<int, GFD_ACT_SILU>{});
+    case GFD_ACT_GELU: return f(std::integral_constant<int, GFD_ACT_GELU>{});
+    default: return f(std::integral_constant<int, GFD_ACT_NONE>{});
+  }
+}
+
+template <typename T, int V, bool BWD, int ACT>
+gfd_status launch(Norm n, const Cut& c, hipStream_t stream) {
   const int vecs = n.channels / V;
-  *team_blocks = 0;
+  int64_t team_blocks = 0;
   if (c.team && n.segments > 0) {
     const int nc = vecs > kMaxTeam ? 2 : 1;
     n.cols = pow2_up((vecs + nc - 1) / nc);
@@ -655,24 +761,30 @@ gfd_status launch(Norm n, const Cut& c, int64_t* team_blocks, hipStream_t stream
     const int teams = block / (n.cols * n.rows);
     int64_t grid = (n.segments + teams - 1) / teams;
     grid = grid < c.teams ? grid : c.teams;
-    *team_blocks = grid;
+    team_blocks = grid;
     const size_t lds = sizeof(double2) * (size_t(block) + size_t(teams) * vecs);
     if (nc == 1)
-      k_team<T, V, 1, BWD><<<int(grid), block, lds, stream>>>(n);
+      k_team<T, V, 1, BWD, ACT><<<int(grid), block, lds, stream>>>(n);
     else if constexpr (V == 1)  // more vectors than threads
-      k_team<T, V, 2, BWD><<<int(grid), block, lds, stream>>>(n);
+      k_team<T, V, 2, BWD, ACT><<<int(grid), block, lds, stream>>>(n);
     GFD_LAUNCH_CHECK();
   }
   if (c.tiled && c.slots > 0) {
     n.cols = pow2_up(vecs < kTileThreads ? vecs : kTileThreads);
     const int64_t tiles = n.ptr ? c.tiles : n.segments * c.tiles;
     const dim3 grid(unsigned(tiles), unsigned((vecs + n.cols - 1) / n.cols));
-    k_sums<T, V, BWD><<<grid, kTileThreads, 0, stream>>>(n);
+    k_sums<T, V, BWD, BWD ? ACT : GFD_ACT_NONE><<<grid, kTileThreads, 0, stream>>>(n);
     GFD_LAUNCH_CHECK();
     const int64_t jobs = n.segments * n.groups;
-    if (jobs > 0) k_stats<T, V, BWD><<<int(jobs < 65536 ? jobs : 65536), kWave, 0, stream>>>(n);
+    const int64_t columns = BWD && (n.dw || n.db) ? (n.channels + 3) / 4 : 0;
+    if (jobs + columns >= (int64_t(1) << 31)) return GFD_ERR_UNSUPPORTED;
+    if (jobs + columns > 0)
+      k_join<T, V, BWD><<<int(jobs + columns), kJoinThreads, 0, stream>>>(n, jobs, c.slots + team_blocks);
     GFD_LAUNCH_CHECK();
-    k_apply<T, V, BWD><<<grid, kTileThreads, 0, stream>>>(n);
+    k_apply<T, V, BWD, ACT><<<grid, kTileThreads, 0, stream>>>(n);
+    GFD_LAUNCH_CHECK();
+  } else if (BWD && (n.dw || n.db)) {
+    k_join<T, V, BWD><<<(n.channels + 3) / 4, kJoinThreads, 0, stream>>>(n, 0, team_blocks);
     GFD_LAUNCH_CHECK();
   }
   return GFD_OK;
@@ -748,7 +860,6 @@ gfd_status gfd_group_norm_fwd(const void* x, int dtype, int64_t segments, int64_
   n.channels = channels;
   n.groups = groups;
   n.w_f32 = w_dtype == GFD_DTYPE_F32;
-  n.act = act;
   n.tile = c.tile;
   n.tiles = int(c.tiles);
   const void* ptrs[] = {x, y};
@@ -756,13 +867,9 @@ gfd_status gfd_group_norm_fwd(const void* x, int dtype, int64_t segments, int64_
     using T = decltype(tag);
     const int v = vector_of(channels / groups, sizeof(T), ptrs, 2, row_stride, ptr ? 0 : seg_stride);
     return with_vector(v, [&](auto w) {
-      constexpr int V = decltype(w)::value;
-      if constexpr (V * sizeof(T) <= 16) {
-        int64_t blocks;
-        return launch<T, V, false>(n, c, &blocks, static_cast<hipStream_t>(stream));
-      } else {
-        return GFD_ERR_UNSUPPORTED;
-      }
+      return with_act(act, [&](auto a) {
+        return launch<T, decltype(w)::value, false, decltype(a)::value>(n, c, static_cast<hipStream_t>(stream));
+      });
     });
   });
 }
@@ -783,58 +890,55 @@ gfd_status gfd_group_norm_bwd(const void* x, int dtype, int64_t segments, int64_
   if (rows && (!x || !grad_y || !grad_x || (!stats && segments > 0) ||
                !aligned_to(grad_y, dtype_size(dtype)) || !aligned_to(grad_x, dtype_size(dtype))))
     return GFD_ERR_ARGUMENT;
-  Cut c = {};
-  Norm n = {};
-  int64_t blocks = 0;
-  if (rows) {
-    c = cut_of(segments, length, ptr != nullptr);
-    if (!grid_ok(c, segments, ptr != nullptr)) return GFD_ERR_UNSUPPORTED;
-    Carve cv(ws, ws_bytes);
-    n.part = cv.take<double2>(size_t(c.slots + c.teams) * channels);
-    n.mom = cv.take<double2>(c.tiled ? size_t(segments) * groups : 0);
-    if (!cv.ok) return GFD_ERR_WORKSPACE;
-    n.x = x;
-    n.dy = grad_y;
-    n.out = grad_x;
-    n.ptr = ptr;
-    n.segments = segments;
-    n.length = length;
-    n.row_stride = row_stride;
-    n.seg_stride = seg_stride;
-    n.w = weight;
-    n.b = bias;
-    n.stats = const_cast<double*>(stats);
+  if (!rows) {  // no row: gradients of 0
+    if (!grad_weight && !grad_bias) return GFD_OK;
+    Norm n = {};
     n.channels = channels;
-    n.groups = groups;
     n.w_f32 = w_dtype == GFD_DTYPE_F32;
-    n.act = act;
-    n.tile = c.tile;
-    n.tiles = int(c.tiles);
-    n.part0 = int(c.slots);
-    const void* ptrs[] = {x, grad_y, grad_x};
-    st = with_dtype(dtype, [&](auto tag) {
-      using T = decltype(tag);
-      const int v = vector_of(channels / groups, sizeof(T), ptrs, 3, row_stride,
-                              ptr ? 0 : seg_stride);
-      return with_vector(v, [&](auto w) {
-        constexpr int V = decltype(w)::value;
-        if constexpr (V * sizeof(T) <= 16) {
-          return launch<T, V, true>(n, c, &blocks, stream);
-        } else {
-          return GFD_ERR_UNSUPPORTED;
-        }
-      });
+    n.dw = grad_weight;
+    n.db = grad_bias;
+    return with_dtype(dtype, [&](auto tag) {
+      k_join<decltype(tag), 1, true><<<(channels + 3) / 4, kJoinThreads, 0, stream>>>(n, 0, 0);
+      GFD_LAUNCH_CHECK();
+      return GFD_OK;
     });
-    if (st != GFD_OK) return st;
   }
-  if (!grad_weight && !grad_bias) return GFD_OK;
+  const Cut c = cut_of(segments, length, ptr != nullptr);
+  if (!grid_ok(c, segments, ptr != nullptr)) return GFD_ERR_UNSUPPORTED;
+  Carve cv(ws, ws_bytes);
+  Norm n = {};
+  n.part = cv.take<double2>(size_t(c.slots + c.teams) * channels);
+  n.mom = cv.take<double2>(c.tiled ? size_t(segments) * groups : 0);
+  if (!cv.ok) return GFD_ERR_WORKSPACE;
+  n.x = x;
+  n.dy = grad_y;
+  n.out = grad_x;
+  n.ptr = ptr;
+  n.segments = segments;
+  n.length = length;
+  n.row_stride = row_stride;
+  n.seg_stride = seg_stride;
+  n.w = weight;
+  n.b = bias;
+  n.stats = const_cast<double*>(stats);
+  n.dw = grad_weight;
+  n.db = grad_bias;
+  n.channels = channels;
+  n.groups = groups;
+  n.w_f32 = w_dtype == GFD_DTYPE_F32;
+  n.tile = c.tile;
+  n.tiles = int(c.tiles);
+  n.part0 = int(c.slots);
+  const void* ptrs[] = {x, grad_y, grad_x};
   return with_dtype(dtype, [&](auto tag) {
     using T = decltype(tag);
-    k_columns<T><<<(channels + 7) / 8, 256, 0, stream>>>(n.part, c.slots + blocks, channels,
-                                                         w_dtype == GFD_DTYPE_F32, grad_weight,
-                                                         grad_bias);
-    GFD_LAUNCH_CHECK();
-    return GFD_OK;
+    const int v = vector_of(channels / groups, sizeof(T), ptrs, 3, row_stride,
+                            ptr ? 0 : seg_stride);
+    return with_vector(v, [&](auto w) {
+      return with_act(act, [&](auto a) {
+        return launch<T, decltype(w)::value, true, decltype(a)::value>(n, c, stream);
+      });
+    });
   });
 }
 

@@ -3,6 +3,8 @@
 // and fp16 elements read and written in vectors, arithmetic in fp32 or fp64.
 #pragma once
 
+#include <type_traits>
+
 #include "gfd_common.h"
 
 namespace gfd {
@@ -25,6 +27,37 @@ template <typename T>
 __device__ __forceinline__ T from_f32(float v) {
   return static_cast<T>(v);
 }
+
+// V elements read as one access and kept in as many registers as they fill (an array of 16-bit
+// elements takes one each)
+template <typename T, int V>
+struct Raw {
+  static constexpr int kWords = (V * int(sizeof(T)) + 3) / 4;
+  uint32_t w[kWords];
+  __device__ __forceinline__ void read(const T* p) {
+    if constexpr (V * sizeof(T) < 4) {
+      w[0] = *reinterpret_cast<const uint16_t*>(p);
+    } else {
+      const auto v = *reinterpret_cast<const Pack<uint32_t, kWords>*>(p);
+#pragma unroll
+      for (int i = 0; i < kWords; ++i) w[i] = v.v[i];
+    }
+  }
+  __device__ __forceinline__ float at(int j) const {  // j: a constant after unrolling
+    if constexpr (sizeof(T) == 4) {
+      return __uint_as_float(w[j]);
+    } else if constexpr (std::is_same<T, bf16_t>::value) {
+      return __uint_as_float(j & 1 ? w[j / 2] & 0xFFFF0000u : w[j / 2] << 16);
+    } else {
+      union {
+        uint16_t u;
+        T f;
+      } h;
+      h.u = uint16_t(j & 1 ? w[j / 2] >> 16 : w[j / 2]);
+      return to_f32(h.f);
+    }
+  }
+};
 
 inline bool aligned_to(const void* p, size_t bytes) {
   return reinterpret_cast<uintptr_t>(p) % bytes == 0;
