@@ -9,6 +9,9 @@
 // dozen operations an element.  A thread holds one vector of V channels of a
 // row, V dividing the channels of a group, so that a vector lies in one group;
 // sums are fp64 throughout (x and x^2: a large mean costs nothing).
+//   * A segment of one row (a node) is its group's lanes' own affair: they exchange
+//     their sums and keep x in registers (k_rows); the backward finds the
+//     statistics again.
 //   * A short segment is normalised by one team of threads (k_team): its rows
 //     are read twice, the second time from cache, in one launch.
 //   * A long one is cut into tiles of rows: k_sums writes each tile's column
@@ -447,6 +450,141 @@ __global__ void __launch_bounds__(kMaxTeam) k_team(const Norm n) {
 }
 
 // ---------------------------------------------------------------------------
+// segments of one row whose groups are 1, 2, 4 .. 64 vectors: the lanes of a group exchange
+// their sums, and x stays in registers
+// ---------------------------------------------------------------------------
+constexpr int kRowThreads = 256;
+constexpr int kRowBlocks = 2048;  // forward; backward: kTeamBlocks, each leaves its column sums
+
+// the sum over the ``width`` (1, 2, 4 .. 64) neighbouring lanes of each such group, in all of them
+__device__ __forceinline__ float near_sum(float v, int width) {
+  auto from = [&](auto ctrl) {
+    return __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), decltype(ctrl)::value, 0xF, 0xF, false));
+  };
+  using std::integral_constant;
+  if (width > 1) v += from(integral_constant<int, 0xB1>{});   // lane ^ 1
+  if (width > 2) v += from(integral_constant<int, 0x4E>{});   // lane ^ 2
+  if (width > 4) v += from(integral_constant<int, 0x141>{});  // mirrored in 8: fours are equal by now
+  if (width > 8) v += from(integral_constant<int, 0x140>{});  // mirrored in 16
+  if (width > 16) v += __shfl_xor(v, 16);
+  if (width > 32) v += __shfl_xor(v, 32);
+  return v;
+}
+
+template <typename T, int V, bool BWD, int ACT>
+__global__ void __launch_bounds__(kRowThreads) k_rows(const Norm n) {
+  constexpr int R = BWD ? 2 : 4;  // rows in flight
+  __shared__ double2 red[kRowThreads];
+  const int vecs = n.channels / V, gv = vecs / n.groups;
+  const int c = threadIdx.x % n.cols, sub = threadIdx.x / n.cols, rows = kRowThreads / n.cols;
+  const int col = blockIdx.y * n.cols + c;
+  const bool on = col < vecs;
+  const float inv = 1.f / float(n.channels / n.groups);
+  float w[V], b[V];
+  affine<T, V>(n.w, n.w_f32, on ? col * V : 0, 1.f, w);
+  affine<T, V>(n.b, n.w_f32, on ? col * V : 0, 0.f, b);
+  double dw[V] = {}, db[V] = {};
+  const int64_t step = int64_t(gridDim.x) * rows;
+  const T* px = static_cast<const T*>(n.x) + col * V;
+  const T* pd = static_cast<const T*>(n.dy) + col * V;
+  T* po = static_cast<T*>(n.out) + col * V;
+  for (int64_t r0 = int64_t(blockIdx.x) * rows + sub; r0 - sub < n.segments; r0 += R * step) {
+    Raw<T, V> x[R], dy[R];
+#pragma unroll
+    for (int u = 0; u < R; ++u) {
+      x[u] = dy[u] = Raw<T, V>{};
+      if (on && r0 + u * step < n.segments) {
+        x[u].read(px + (r0 + u * step) * n.seg_stride);
+        if (BWD) dy[u].read(pd + (r0 + u * step) * n.channels);
+      }
+    }
+    float e[V] = {}, f[V] = {};
+#pragma unroll
+    for (int u = 0; u < R; ++u) {
+      // the mean in two steps: about a first one, which rounding leaves a little off, d is small
+      float d[V], s = 0.f;
+#pragma unroll
+      for (int j = 0; j < V; ++j) s += x[u].at(j);
+      const float m = near_sum(s, gv) * inv;
+      float s1 = 0.f, s2 = 0.f;
+#pragma unroll
+      for (int j = 0; j < V; ++j) {
+        d[j] = x[u].at(j) - m;
+        s1 += d[j];
+        s2 = fmaf(d[j], d[j], s2);
+      }
+      const float off = near_sum(s1, gv) * inv;
+      const float var = fmaxf(fmaf(-off, off, near_sum(s2, gv) * inv), 0.f);
+      const float r = rsqrtf(var + float(n.eps)), lr = off * r;
+      float xh[V], z[V];
+      bool near = false;
+#pragma unroll
+      for (int j = 0; j < V; ++j) {
+        xh[j] = fmaf(d[j], r, -lr);
+        z[j] = fmaf(xh[j], w[j], b[j]);
+        if (ACT == GFD_ACT_RELU) near = near || fabsf(z[j]) <= 4e-6f * (fabsf(xh[j] * w[j]) + fabsf(b[j]));
+      }
+      if (ACT == GFD_ACT_RELU && __ballot(near)) {  // relu's side from fp64
+        double ds = 0.0, dq = 0.0;
+#pragma unroll
+        for (int j = 0; j < V; ++j) {
+          ds += double(x[u].at(j));
+          dq += double(x[u].at(j)) * double(x[u].at(j));
+        }
+        for (int k = 1; k < gv; k <<= 1) {
+          ds += __shfl_xor(ds, k);
+          dq += __shfl_xor(dq, k);
+        }
+        const double2 mm = moments_of(ds, dq, double(n.channels / n.groups), n.eps);
+        if (near) {
+#pragma unroll
+          for (int j = 0; j < V; ++j)
+            z[j] = float((double(x[u].at(j)) - mm.x) * mm.y * double(w[j]) + double(b[j]));
+        }
+      }
+      Pack<T, V> o;
+      if (BWD) {
+        float dz[V], sa = 0.f, sb = 0.f;
+#pragma unroll
+        for (int j = 0; j < V; ++j) {
+          float g;
+          activate<ACT>(z[j], &g);
+          dz[j] = dy[u].at(j) * g;
+          const float wd = w[j] * dz[j];
+          sa += wd;
+          sb = fmaf(wd, xh[j], sb);
+          e[j] += dz[j];
+          f[j] = fmaf(dz[j], xh[j], f[j]);
+        }
+        const float ma = near_sum(sa, gv) * inv, mb = near_sum(sb, gv) * inv;
+#pragma unroll
+        for (int j = 0; j < V; ++j) o.v[j] = from_f32<T>(r * (fmaf(w[j], dz[j], -ma) - xh[j] * mb));
+      } else {
+#pragma unroll
+        for (int j = 0; j < V; ++j) o.v[j] = from_f32<T>(activate<ACT>(z[j], nullptr));
+      }
+      if (on && r0 + u * step < n.segments)
+        *reinterpret_cast<Pack<T, V>*>(po + (r0 + u * step) * n.channels) = o;
+    }
+    if (BWD) {
+#pragma unroll
+      for (int j = 0; j < V; ++j) {
+        db[j] += double(e[j]);
+        dw[j] += double(f[j]);
+      }
+    }
+  }
+  if (BWD) {
+    double2* part = n.part + int64_t(blockIdx.x) * n.channels;
+#pragma unroll
+    for (int j = 0; j < V; ++j) {
+      const double2 v = sum_rows({db[j], dw[j]}, n.cols, red);
+      if (threadIdx.x < n.cols && on) part[col * V + j] = v;
+    }
+  }
+}
+
+// ---------------------------------------------------------------------------
 // long segments
 // ---------------------------------------------------------------------------
 constexpr int kTileThreads = 256;
@@ -750,7 +888,16 @@ template <typename T, int V, bool BWD, int ACT>
 gfd_status launch(Norm n, const Cut& c, hipStream_t stream) {
   const int vecs = n.channels / V;
   int64_t team_blocks = 0;
-  if (c.team && n.segments > 0) {
+  const int gv = vecs / n.groups;
+  if (!n.ptr && n.length == 1 && gv <= kWave && (gv & (gv - 1)) == 0) {
+    n.cols = pow2_up(vecs < kWave ? vecs : kWave);
+    const int rows = kRowThreads / n.cols;
+    const int64_t need = (n.segments + rows - 1) / rows, most = BWD ? c.teams : kRowBlocks;
+    team_blocks = need < most ? need : most;
+    k_rows<T, V, BWD, ACT><<<dim3(unsigned(team_blocks), unsigned((vecs + n.cols - 1) / n.cols)),
+                             kRowThreads, 0, stream>>>(n);
+    GFD_LAUNCH_CHECK();
+  } else if (c.team && n.segments > 0) {
     const int nc = vecs > kMaxTeam ? 2 : 1;
     n.cols = pow2_up((vecs + nc - 1) / nc);
     const int block = n.cols > 256 ? n.cols : 256;
@@ -855,7 +1002,10 @@ gfd_status gfd_group_norm_fwd(const void* x, int dtype, int64_t segments, int64_
   n.w = weight;
   n.b = bias;
   // the tile kernels hand the statistics on: without a place of the caller's, through ``mom``
-  n.stats = stats ? stats : c.tiled ? reinterpret_cast<double*>(n.mom) : nullptr;
+  n.stats = !ptr && length == 1 ? nullptr
+            : stats             ? stats
+            : c.tiled           ? reinterpret_cast<double*>(n.mom)
+                                : nullptr;
   n.eps = eps;
   n.channels = channels;
   n.groups = groups;
@@ -877,7 +1027,7 @@ gfd_status gfd_group_norm_fwd(const void* x, int dtype, int64_t segments, int64_
 gfd_status gfd_group_norm_bwd(const void* x, int dtype, int64_t segments, int64_t length,
                               const int64_t* ptr, int channels, int groups, int64_t row_stride,
                               int64_t seg_stride, const void* weight, const void* bias,
-                              int w_dtype, int act, const double* stats, const void* grad_y,
+                              int w_dtype, double eps, int act, const double* stats, const void* grad_y,
                               void* grad_x, void* grad_weight, void* grad_bias, void* ws,
                               size_t ws_bytes, gfd_stream_t stream_) {
   hipStream_t stream = static_cast<hipStream_t>(stream_);
@@ -886,8 +1036,9 @@ gfd_status gfd_group_norm_bwd(const void* x, int dtype, int64_t segments, int64_
   if (st != GFD_OK) return st;
   if (!aligned_to(grad_weight, dtype_size(w_dtype)) || !aligned_to(grad_bias, dtype_size(w_dtype)))
     return GFD_ERR_ARGUMENT;
+  if (!(eps >= 0.0)) return GFD_ERR_ARGUMENT;
   const bool rows = length > 0 && (ptr || segments > 0);
-  if (rows && (!x || !grad_y || !grad_x || (!stats && segments > 0) ||
+  if (rows && (!x || !grad_y || !grad_x || (!stats && segments > 0 && (ptr || length > 1)) ||
                !aligned_to(grad_y, dtype_size(dtype)) || !aligned_to(grad_x, dtype_size(dtype))))
     return GFD_ERR_ARGUMENT;
   if (!rows) {  // no row: gradients of 0
@@ -920,7 +1071,9 @@ gfd_status gfd_group_norm_bwd(const void* x, int dtype, int64_t segments, int64_
   n.seg_stride = seg_stride;
   n.w = weight;
   n.b = bias;
-  n.stats = const_cast<double*>(stats);
+  // a row of its own: its statistics are found again, which is less than reading them
+  n.stats = !ptr && length == 1 ? nullptr : const_cast<double*>(stats);
+  n.eps = eps;
   n.dw = grad_weight;
   n.db = grad_bias;
   n.channels = channels;

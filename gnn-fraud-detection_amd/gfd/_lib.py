@@ -141,7 +141,7 @@ SIGNATURES = {
     "gfd_group_norm_fwd": (c_i32, [P, ct.c_int, c_i64, c_i64, P, ct.c_int, ct.c_int, c_i64, c_i64,
                                    P, P, ct.c_int, c_f64, ct.c_int, P, P, P, c_sz, P]),
     "gfd_group_norm_bwd": (c_i32, [P, ct.c_int, c_i64, c_i64, P, ct.c_int, ct.c_int, c_i64, c_i64,
-                                   P, P, ct.c_int, ct.c_int, P, P, P, P, P, P, c_sz, P]),
+                                   P, P, ct.c_int, c_f64, ct.c_int, P, P, P, P, P, P, c_sz, P]),
     "gfd_class_logp_workspace_size": (c_sz, [c_i64, c_i64, ct.c_int]),
     "gfd_class_logp_fwd": (c_i32, [P, ct.c_int, c_i64, c_i64, c_i64, P, c_i64, ct.c_int, P, P, P,
                                    P, P, P, c_sz, P]),

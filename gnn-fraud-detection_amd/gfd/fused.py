@@ -395,7 +395,8 @@ def _check_rows(what: str, name: str, t: torch.Tensor) -> None:
 
 class _GroupNorm(torch.autograd.Function):
     """act(group_norm(x)) over gfd_group_norm_fwd / _bwd; x [B, L, C] (dense) or
-    [N, C] with ptr (ragged).  x and the fp64 statistics are kept."""
+    [N, C] with ptr (ragged).  x and, but for single rows, the fp64 statistics are
+    kept."""
 
     @staticmethod
     def forward(ctx, x, weight, bias, ptr, groups, eps, act, grad_mode):
@@ -404,8 +405,9 @@ class _GroupNorm(torch.autograd.Function):
         segments, length = (ptr.numel() - 1, x.size(0)) if ragged else (x.size(0), x.size(1))
         keep = grad_mode and any(ctx.needs_input_grad[:3])
         y = torch.empty(x.shape, dtype=x.dtype, device=dev)
-        stats = (torch.empty((segments, groups, 2), dtype=torch.float64, device=dev) if keep
-                 else None)
+        # a row of its own keeps no statistics: the backward finds them again
+        stats = (torch.empty((segments, groups, 2), dtype=torch.float64, device=dev)
+                 if keep and (ragged or length != 1) else None)
         ctx.geom = (_ROW_DTYPES[x.dtype], segments, length, _lib.ptr(ptr), C, groups,
                     x.stride(-2), 0 if ragged else x.stride(0))
         w_dtype = _ROW_DTYPES[weight.dtype if weight is not None else
@@ -418,7 +420,7 @@ class _GroupNorm(torch.autograd.Function):
                      _lib.ptr(ws), nbytes, _lib.stream_handle(dev))
         if keep:
             ctx.save_for_backward(x, weight, bias, ptr, stats)
-            ctx.act, ctx.w_dtype = act, w_dtype
+            ctx.act, ctx.w_dtype, ctx.eps = act, w_dtype, eps
         return y
 
     @staticmethod
@@ -436,7 +438,7 @@ class _GroupNorm(torch.autograd.Function):
                                                    groups, 1)
         ws = _ws(nbytes, dev)
         _lib.call_on(dev, "gfd_group_norm_bwd", x.data_ptr(), *ctx.geom, _lib.ptr(weight),
-                     _lib.ptr(bias), ctx.w_dtype, ctx.act, stats.data_ptr(), grad.data_ptr(),
+                     _lib.ptr(bias), ctx.w_dtype, ctx.eps, ctx.act, _lib.ptr(stats), grad.data_ptr(),
                      gx.data_ptr(), _lib.ptr(gw), _lib.ptr(gb), ws.data_ptr(), ws.numel(),
                      _lib.stream_handle(dev))
         return gx, gw, gb, None, None, None, None, None

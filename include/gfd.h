@@ -601,7 +601,8 @@ gfd_status gfd_rows_copy(const float* src, int64_t src_stride, const int32_t* sr
  * grad_x) contiguous in the rows' order.  weight / bias [channels], nullable
  * (identity), w_dtype F32 or x's.  Statistics and sums are fp64; stats (fp64
  * [segments, groups, 2] = mean, 1/sqrt(var + eps)) is nullable in the forward
- * and what the backward takes.  channels <= 2048 and a multiple of groups.
+ * and what the backward takes; dense segments of one row keep none (stats NULL:
+ * the backward finds them again).  channels <= 2048 and a multiple of groups.
  * GELU is the erf form.  relu's side is decided in fp64 where fp32 cannot
  * tell it.  grad_weight / grad_bias (w_dtype, nullable) are deterministic.
  * ws: gfd_group_norm_workspace_size bytes (may be 0: ws may then be NULL).
@@ -620,7 +621,8 @@ gfd_status gfd_group_norm_fwd(const void* x, int dtype, int64_t segments, int64_
 gfd_status gfd_group_norm_bwd(const void* x, int dtype, int64_t segments, int64_t length,
                               const int64_t* ptr, int channels, int groups, int64_t row_stride,
                               int64_t seg_stride, const void* weight, const void* bias,
-                              int w_dtype, int act, const double* stats, const void* grad_y,
+                              int w_dtype, double eps, int act, const double* stats,
+                              const void* grad_y,
                               void* grad_x, void* grad_weight, void* grad_bias, void* ws,
                               size_t ws_bytes, gfd_stream_t stream);
 
