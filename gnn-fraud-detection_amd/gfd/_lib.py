@@ -216,4 +216,7 @@ def ptr(t) -> int | None:
 
 def stream_handle(device=None) -> int:
     import torch
+    raw = getattr(torch._C, "_cuda_getCurrentRawStream", None)   # 2 us less than a Stream object
+    if raw is not None and device is not None and getattr(device, "index", None) is not None:
+        return raw(device.index)
     return torch.cuda.current_stream(device).cuda_stream

@@ -393,34 +393,36 @@ def _check_rows(what: str, name: str, t: torch.Tensor) -> None:
         raise TypeError(f"gfd {what}: {name} must be float32, bfloat16 or float16 (got {t.dtype})")
 
 
+def _group_norm_fwd(x, weight, bias, ptr, groups, eps, act, keep):
+    """(y, statistics or None, the leading arguments of the C calls, GFD_DTYPE_* of the affine)."""
+    dev, ragged, C = x.device, ptr is not None, x.size(-1)
+    segments, length = (ptr.numel() - 1, x.size(0)) if ragged else (x.size(0), x.size(1))
+    y = torch.empty(x.shape, dtype=x.dtype, device=dev)
+    # a row of its own keeps no statistics: the backward finds them again
+    stats = (torch.empty((segments, groups, 2), dtype=torch.float64, device=dev)
+             if keep and (ragged or length != 1) else None)
+    geom = (_ROW_DTYPES[x.dtype], segments, length, _lib.ptr(ptr), C, groups, x.stride(-2),
+            0 if ragged else x.stride(0))
+    w_dtype = _ROW_DTYPES[weight.dtype if weight is not None else
+                          bias.dtype if bias is not None else x.dtype]
+    nbytes = _lib.load().gfd_group_norm_workspace_size(segments, length, int(ragged), C, groups, 0)
+    ws = _ws(nbytes, dev) if nbytes else None
+    _lib.call_on(dev, "gfd_group_norm_fwd", x.data_ptr(), *geom, _lib.ptr(weight), _lib.ptr(bias),
+                 w_dtype, eps, act, y.data_ptr(), _lib.ptr(stats), _lib.ptr(ws), nbytes,
+                 _lib.stream_handle(dev))
+    return y, stats, geom, w_dtype
+
+
 class _GroupNorm(torch.autograd.Function):
     """act(group_norm(x)) over gfd_group_norm_fwd / _bwd; x [B, L, C] (dense) or
     [N, C] with ptr (ragged).  x and, but for single rows, the fp64 statistics are
     kept."""
 
     @staticmethod
-    def forward(ctx, x, weight, bias, ptr, groups, eps, act, grad_mode):
-        dev, ragged = x.device, ptr is not None
-        C = x.size(-1)
-        segments, length = (ptr.numel() - 1, x.size(0)) if ragged else (x.size(0), x.size(1))
-        keep = grad_mode and any(ctx.needs_input_grad[:3])
-        y = torch.empty(x.shape, dtype=x.dtype, device=dev)
-        # a row of its own keeps no statistics: the backward finds them again
-        stats = (torch.empty((segments, groups, 2), dtype=torch.float64, device=dev)
-                 if keep and (ragged or length != 1) else None)
-        ctx.geom = (_ROW_DTYPES[x.dtype], segments, length, _lib.ptr(ptr), C, groups,
-                    x.stride(-2), 0 if ragged else x.stride(0))
-        w_dtype = _ROW_DTYPES[weight.dtype if weight is not None else
-                              bias.dtype if bias is not None else x.dtype]
-        lib = _lib.load()
-        nbytes = lib.gfd_group_norm_workspace_size(segments, length, int(ragged), C, groups, 0)
-        ws = _ws(nbytes, dev) if nbytes else None
-        _lib.call_on(dev, "gfd_group_norm_fwd", x.data_ptr(), *ctx.geom, _lib.ptr(weight),
-                     _lib.ptr(bias), w_dtype, eps, act, y.data_ptr(), _lib.ptr(stats),
-                     _lib.ptr(ws), nbytes, _lib.stream_handle(dev))
-        if keep:
-            ctx.save_for_backward(x, weight, bias, ptr, stats)
-            ctx.act, ctx.w_dtype, ctx.eps = act, w_dtype, eps
+    def forward(ctx, x, weight, bias, ptr, groups, eps, act):
+        y, stats, ctx.geom, ctx.w_dtype = _group_norm_fwd(x, weight, bias, ptr, groups, eps, act, True)
+        ctx.save_for_backward(x, weight, bias, ptr, stats)
+        ctx.act, ctx.eps = act, eps
         return y
 
     @staticmethod
@@ -441,7 +443,11 @@ class _GroupNorm(torch.autograd.Function):
                      _lib.ptr(bias), ctx.w_dtype, ctx.eps, ctx.act, _lib.ptr(stats), grad.data_ptr(),
                      gx.data_ptr(), _lib.ptr(gw), _lib.ptr(gb), ws.data_ptr(), ws.numel(),
                      _lib.stream_handle(dev))
-        return gx, gw, gb, None, None, None, None, None
+        return gx, gw, gb, None, None, None, None
+
+
+def _needs_grad(*tensors) -> bool:
+    return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)
 
 
 def group_norm(x: torch.Tensor, num_groups: int, weight: Optional[torch.Tensor] = None,
@@ -491,8 +497,9 @@ def group_norm(x: torch.Tensor, num_groups: int, weight: Optional[torch.Tensor] 
         x = x.contiguous()
     weight = weight.contiguous() if weight is not None else None
     bias = bias.contiguous() if bias is not None else None
-    return _GroupNorm.apply(x, weight, bias, ptr, int(num_groups), float(eps), ACTIVATIONS[act],
-                            torch.is_grad_enabled()).view(shape)
+    args = (x, weight, bias, ptr, int(num_groups), float(eps), ACTIVATIONS[act])
+    y = _GroupNorm.apply(*args) if _needs_grad(x, weight, bias) else _group_norm_fwd(*args, False)[0]
+    return y if y.shape == shape else y.view(shape)
 
 
 class ClassLogProbs(NamedTuple):
@@ -503,27 +510,34 @@ class ClassLogProbs(NamedTuple):
     top_classes: torch.Tensor            # [..., top]
 
 
+def _class_log_probs_fwd(logits, target, top, ignore_index):
+    """(logp, entropy, top_logp, top_class, statistics, the leading arguments of the C calls)."""
+    dev = logits.device
+    rows, classes = logits.shape
+    f32 = dict(dtype=torch.float32, device=dev)
+    logp = torch.empty(rows, **f32) if target is not None else None
+    entropy = torch.empty(rows, **f32)
+    top_logp = torch.empty((rows, top), **f32)
+    top_class = torch.empty((rows, top), dtype=torch.int64, device=dev)
+    stats = torch.empty((rows, 2), **f32)
+    nbytes = _lib.load().gfd_class_logp_workspace_size(rows, classes, top)
+    ws = _ws(nbytes, dev) if nbytes else None
+    geom = (_ROW_DTYPES[logits.dtype], rows, classes, logits.stride(0))
+    _lib.call_on(dev, "gfd_class_logp_fwd", logits.data_ptr(), *geom, _lib.ptr(target),
+                 ignore_index, top, _lib.ptr(logp), entropy.data_ptr(), top_logp.data_ptr(),
+                 top_class.data_ptr(), stats.data_ptr(), _lib.ptr(ws), nbytes,
+                 _lib.stream_handle(dev))
+    return logp, entropy, top_logp, top_class, stats, geom
+
+
 class _ClassLogProbs(torch.autograd.Function):
     """Over gfd_class_logp_fwd / _bwd: the logits, two statistics and the entropy
     of a row are kept."""
 
     @staticmethod
     def forward(ctx, logits, target, top, ignore_index):
-        dev = logits.device
-        rows, classes = logits.shape
-        f32 = dict(dtype=torch.float32, device=dev)
-        logp = torch.empty(rows, **f32) if target is not None else None
-        entropy = torch.empty(rows, **f32)
-        top_logp = torch.empty((rows, top), **f32)
-        top_class = torch.empty((rows, top), dtype=torch.int64, device=dev)
-        stats = torch.empty((rows, 2), **f32)
-        nbytes = _lib.load().gfd_class_logp_workspace_size(rows, classes, top)
-        ws = _ws(nbytes, dev) if nbytes else None
-        ctx.geom = (_ROW_DTYPES[logits.dtype], rows, classes, logits.stride(0))
-        _lib.call_on(dev, "gfd_class_logp_fwd", logits.data_ptr(), *ctx.geom, _lib.ptr(target),
-                     ignore_index, top, _lib.ptr(logp), entropy.data_ptr(), top_logp.data_ptr(),
-                     top_class.data_ptr(), stats.data_ptr(), _lib.ptr(ws), nbytes,
-                     _lib.stream_handle(dev))
+        logp, entropy, top_logp, top_class, stats, ctx.geom = _class_log_probs_fwd(
+            logits, target, top, ignore_index)
         ctx.save_for_backward(logits, target, entropy, top_class, stats)
         ctx.top, ctx.ignore_index = top, ignore_index
         ctx.mark_non_differentiable(top_class)
@@ -576,7 +590,9 @@ def class_log_probs(logits: torch.Tensor, target: Optional[torch.Tensor] = None,
     x = logits if logits.dim() == 2 else logits.reshape(-1, classes)
     if (classes > 1 and x.stride(1) != 1) or x.stride(0) < 0:
         x = x.contiguous()
-    logp, entropy, top_logp, top_class = _ClassLogProbs.apply(x, target, int(top), int(ignore_index))
+    args = (x, target, int(top), int(ignore_index))
+    logp, entropy, top_logp, top_class = (_ClassLogProbs.apply(*args) if _needs_grad(x) else
+                                          _class_log_probs_fwd(*args)[:4])
     if logits.dim() == 2:
         return ClassLogProbs(logp, entropy, top_logp, top_class)
     return ClassLogProbs(logp.view(lead) if logp is not None else None, entropy.view(lead),
