@@ -50,7 +50,8 @@ struct Norm {
   int tile;        // rows of a tile; ragged segments up to it are short
   int tiles;       // of one segment (dense) or of all rows (ragged)
   int part0;       // first row of ``part`` that the teams write (backward)
-  int cols, rows;  // team: threads over a row's vectors, over rows
+  int cols, rows;  // threads over a row's vectors and over rows, powers of two
+  int cols2, rows2;  // their logarithms
   int zero_rest;   // ragged: k_apply clears the rows of no segment
 };
 
@@ -89,40 +90,25 @@ __device__ __forceinline__ int64_t segment_of(const Norm& n, int64_t r) {
 }
 
 struct Piece {
-  int64_t seg, r0, r1;  // rows [r0, r1) of segment seg
+  int64_t seg, r0, r1;  // rows [r0, r1) of segment seg, none where r0 >= r1
 };
 
-// the pieces of long segments in a tile; piece i's sums go to row 2 t + i (ragged) or t of ``part``
-__device__ __forceinline__ int pieces_of(const Norm& n, int64_t t, Piece (&p)[2]) {
-  if (!n.ptr) {
-    const int64_t s = t / n.tiles, r0 = s * n.length, k = (t - s * n.tiles) * n.tile;
-    const int64_t k1 = k + n.tile < n.length ? k + n.tile : n.length;
-    p[0] = {s, r0 + k, r0 + k1};
-    return 1;
-  }
+// piece i (ragged: 0 or 1) of the long segments in tile t; its sums go to row 2 t + i (ragged) or
+// seg * tiles + t of ``part``
+__device__ __forceinline__ Piece piece_of(const Norm& n, int64_t t, int i) {
   const int64_t a = t * n.tile, e = a + n.tile < n.length ? a + n.tile : n.length;
-  int found = 0;
-  auto piece = [&](int i, int64_t s) {
-    int64_t r0, r1;
-    segment_rows(n, s, r0, r1);
-    const int64_t to = r1;
-    p[i] = {-1, 0, 0};
-    if (r1 - r0 > n.tile) {
-      r0 = r0 < a ? a : r0;
-      r1 = r1 > e ? e : r1;
-      if (r0 < r1) {
-        p[i] = {s, r0, r1};
-        found = i + 1;
-      }
-    }
-    return to;
-  };
-  const int64_t s0 = segment_of(n, a);
-  p[0] = p[1] = {-1, 0, 0};
-  if (s0 >= 0 && piece(0, s0) >= e) return found;
-  const int64_t s1 = segment_of(n, e - 1);
-  if (s1 >= 0 && s1 != s0) piece(1, s1);
-  return found;
+  if (!n.ptr) {
+    const int64_t s = blockIdx.z, base = s * n.length;
+    return {s, base + a, base + e};
+  }
+  Piece p = {segment_of(n, i == 0 ? a : e - 1), 0, 0};
+  if (p.seg < 0) return p;
+  segment_rows(n, p.seg, p.r0, p.r1);
+  // the second is the one that starts inside the tile
+  if (p.r1 - p.r0 <= n.tile || (i == 1 && p.r0 <= a)) p.r1 = p.r0;
+  p.r0 = p.r0 < a ? a : p.r0;
+  p.r1 = p.r1 > e ? e : p.r1;
+  return p;
 }
 
 template <typename T>
@@ -282,6 +268,32 @@ __device__ __forceinline__ double2 sum_rows(double2 v, int cols, double2* red) {
   return v;
 }
 
+// A thread's sums of x and x^2, in fp32 about its own first element k and, every few rows, into
+// fp64 (a conversion to fp64 takes four times an fp32 operation): what rounding does to the
+// deviations from k, however far k lies from 0, is not multiplied by it.  The squares of the k -
+// mean of all threads are at most the sum of squares itself, so neither does an odd k cost digits.
+struct Shifted {
+  float k = 0.f, s = 0.f, q = 0.f;
+  double a = 0.0, b = 0.0;
+  int64_t n = 0;
+  __device__ __forceinline__ void add(float x) {
+    const float d = x - k;
+    s += d;
+    q = fmaf(d, d, q);
+  }
+  __device__ __forceinline__ void fold(int count) {
+    a += double(s);
+    b += double(q);
+    s = q = 0.f;
+    n += count;
+  }
+  // the sums themselves
+  __device__ __forceinline__ double2 sums() const {
+    const double c = double(k), m = double(n);
+    return {fma(m, c, a), fma(c, fma(m, c, 2.0 * a), b)};
+  }
+};
+
 // ---------------------------------------------------------------------------
 // short segments: a team of cols x rows threads each
 // ---------------------------------------------------------------------------
@@ -292,8 +304,8 @@ __global__ void __launch_bounds__(kMaxTeam) k_team(const Norm n) {
   double2* col_sum = lds + blockDim.x;  // [teams][vecs]
   using P = Pack<T, V>;
   const int vecs = n.channels / V, gv = vecs / n.groups;
-  const int size = n.cols * n.rows, teams = blockDim.x / size;
-  const int c = threadIdx.x % n.cols, tr = threadIdx.x / n.cols % n.rows, team = threadIdx.x / size;
+  const int size2 = n.cols2 + n.rows2, teams = blockDim.x >> size2;
+  const int c = threadIdx.x & (n.cols - 1), tr = threadIdx.x >> n.cols2 & (n.rows - 1), team = threadIdx.x >> size2;
   double dw[NC][V] = {}, db[NC][V] = {};
   for (int64_t s0 = int64_t(blockIdx.x) * teams; s0 < n.segments; s0 += int64_t(gridDim.x) * teams) {
     auto rows_of = [&](int64_t s, int64_t& r0, int64_t& r1) {
@@ -358,15 +370,17 @@ __global__ void __launch_bounds__(kMaxTeam) k_team(const Norm n) {
     if (!kept)
       reduce(
           [&](int, int col, double& a, double& b) {
+            Shifted t;
             for (int64_t r = r0 + tr; r < r1; r += n.rows) {
               const Raw<T, V> x = x_at(r, col);
+              if (t.n == 0) t.k = x.at(0);
 #pragma unroll
-              for (int j = 0; j < V; ++j) {
-                const double v = double(x.at(j));
-                a += v;
-                b += v * v;
-              }
+              for (int j = 0; j < V; ++j) t.add(x.at(j));
+              t.fold(V);
             }
+            const double2 v = t.sums();
+            a = v.x;
+            b = v.y;
           },
           [&](int64_t s, int g, double a, double b, double count) {
             const double2 m = moments_of(a, b, count, n.eps);
@@ -394,16 +408,18 @@ __global__ void __launch_bounds__(kMaxTeam) k_team(const Norm n) {
       reduce(
           [&](int k, int col, double& a, double& b) {
             for (int64_t r = r0 + tr; r < r1; r += n.rows) {
-              float dz[V], xh[V];
+              float dz[V], xh[V], sa = 0.f, sb = 0.f;
               cols[k].slope(n, x_at(r, col), dy_at(r, col), dz, xh);
 #pragma unroll
               for (int j = 0; j < V; ++j) {
-                const double e = double(dz[j]), f = double(dz[j] * xh[j]);
-                db[k][j] += e;
-                dw[k][j] += f;
-                a += double(cols[k].A[j]) * e;  // r times w
-                b += double(cols[k].A[j]) * f;
+                const float f = dz[j] * xh[j];
+                db[k][j] += double(dz[j]);
+                dw[k][j] += double(f);
+                sa = fmaf(cols[k].A[j], dz[j], sa);  // r times w
+                sb = fmaf(cols[k].A[j], f, sb);
               }
+              a += double(sa);
+              b += double(sb);
             }
           },
           [&](int64_t, int, double a, double b, double count) { return double2{a / count, b / count}; });
@@ -476,7 +492,7 @@ __global__ void __launch_bounds__(kRowThreads) k_rows(const Norm n) {
   constexpr int R = BWD ? 2 : 4;  // rows in flight
   __shared__ double2 red[kRowThreads];
   const int vecs = n.channels / V, gv = vecs / n.groups;
-  const int c = threadIdx.x % n.cols, sub = threadIdx.x / n.cols, rows = kRowThreads / n.cols;
+  const int c = threadIdx.x & (n.cols - 1), sub = threadIdx.x >> n.cols2, rows = kRowThreads >> n.cols2;
   const int col = blockIdx.y * n.cols + c;
   const bool on = col < vecs;
   const float inv = 1.f / float(n.channels / n.groups);
@@ -590,47 +606,66 @@ __global__ void __launch_bounds__(kRowThreads) k_rows(const Norm n) {
 constexpr int kTileThreads = 256;
 
 // column sums of a tile: forward [slot][vecs] of x and x^2, backward [slot][channels] of dz and
-// dz xhat; ragged tiles have two slots, an unused one is 0
+// dz xhat; ragged tiles have two slots, an unused one is 0.  (These kernels are kept small: the
+// first wave of a CU waits about 0.1 us for every 64 bytes of its instructions, which for a few
+// MB of rows is most of the time.)
 template <typename T, int V, bool BWD, int ACT>
 __global__ void __launch_bounds__(kTileThreads) k_sums(const Norm n) {
   constexpr int S = BWD ? V : 1;
-  constexpr int R = BWD ? 4 : 8;  // rows in flight
+  constexpr int R = BWD ? 2 : 8;  // rows in flight
   __shared__ double2 red[kTileThreads];
   const int vecs = n.channels / V, gv = vecs / n.groups;
-  const int c = threadIdx.x % n.cols, tr = threadIdx.x / n.cols, rows = kTileThreads / n.cols;
+  const int c = threadIdx.x & (n.cols - 1), tr = threadIdx.x >> n.cols2, rows = kTileThreads >> n.cols2;
   const int col = blockIdx.y * n.cols + c;
+  const bool on = col < vecs;
   const int64_t t = blockIdx.x;
-  Piece p[2];
-  const int found = pieces_of(n, t, p);
 #pragma unroll 1
   for (int i = 0; i < (n.ptr ? 2 : 1); ++i) {
-    const bool here = i < found && p[i].seg >= 0;
+    const Piece p = piece_of(n, t, i);
     double a[S] = {}, b[S] = {};
-    if (here && col < vecs) {
+    if (on && p.r0 < p.r1) {
       Columns<T, V, ACT> k;
       if (BWD) {
-        const double* st = n.stats + 2 * (p[i].seg * n.groups + col / gv);
+        const double* st = n.stats + 2 * (p.seg * n.groups + col / gv);
         k.set(n, col, st[0], st[1]);
       }
-      const T* px = row_in<T>(n, n.x, p[i].seg, p[i].r0 + tr) + col * V;
-      const T* pd = static_cast<const T*>(n.dy) + (p[i].r0 + tr) * n.channels + col * V;
-      const int64_t xs = rows * n.row_stride, ds = int64_t(rows) * n.channels;
-      int64_t left = p[i].r1 - p[i].r0 - tr;
-      auto take = [&](auto number) {  // that many rows, all of them read first
-        constexpr int N = decltype(number)::value;
-        Raw<T, V> x[N], dy[N];
+      Shifted t1;
+      float e[V] = {}, f[V] = {};  // of a few rows, in fp32
+      int held = 0;
+      auto fold = [&]() {
 #pragma unroll
-        for (int u = 0; u < N; ++u) {
-          x[u].read(px + u * xs);
-          if (BWD) dy[u].read(pd + u * ds);
+        for (int j = 0; j < V; ++j) {
+          a[j % S] += double(e[j]);
+          b[j % S] += double(f[j]);
+          e[j] = f[j] = 0.f;
         }
-        px += N * xs;
-        pd += N * ds;
-        left -= N * rows;
-        if (BWD) {
-          float e[V] = {}, f[V] = {};  // of N rows in fp32
+        held = 0;
+      };
+      const T* px = row_in<T>(n, n.x, p.seg, p.r0 + tr) + col * V;
+      const T* pd = static_cast<const T*>(n.dy) + (p.r0 + tr) * n.channels + col * V;
+      const int64_t xs = rows * n.row_stride, ds = int64_t(rows) * n.channels;
+      int left = int(p.r1 - p.r0) - tr;
+      if (!BWD && left > 0) {
+        Raw<T, V> x;
+        x.read(px);
+        t1.k = x.at(0);
+      }
+#pragma unroll 1
+      for (; left > 0; left -= R * rows) {
+        Raw<T, V> x[R], dy[R];
 #pragma unroll
-          for (int u = 0; u < N; ++u) {
+        for (int u = 0; u < R; ++u) {
+          x[u] = dy[u] = Raw<T, V>{};
+          if (u * rows < left) {
+            x[u].read(px + u * xs);
+            if (BWD) dy[u].read(pd + u * ds);
+          }
+        }
+        px += R * xs;
+        pd += R * ds;
+        if (BWD) {  // a row beyond the last adds 0 (dy is 0)
+#pragma unroll
+          for (int u = 0; u < R; ++u) {
             float dz[V], xh[V];
             k.slope(n, x[u], dy[u], dz, xh);
 #pragma unroll
@@ -639,31 +674,32 @@ __global__ void __launch_bounds__(kTileThreads) k_sums(const Norm n) {
               f[j] = fmaf(dz[j], xh[j], f[j]);
             }
           }
-#pragma unroll
-          for (int j = 0; j < V; ++j) {
-            a[j % S] += double(e[j]);
-            b[j % S] += double(f[j]);
-          }
+          if ((held += R) >= 32) fold();
         } else {
 #pragma unroll
-          for (int u = 0; u < N; ++u)
+          for (int u = 0; u < R; ++u)
+            if (u * rows < left) {
 #pragma unroll
-            for (int j = 0; j < V; ++j) {
-              const double v = double(x[u].at(j));
-              a[0] += v;
-              b[0] += v * v;
+              for (int j = 0; j < V; ++j) t1.add(x[u].at(j));
             }
+          t1.fold(V * (left > (R - 1) * rows ? R : (left + rows - 1) / rows));
         }
-      };
-      while (left > (R - 1) * rows) take(std::integral_constant<int, R>{});
-      while (left > 0) take(std::integral_constant<int, 1>{});
+      }
+      if (BWD) {
+        fold();
+      } else {
+        const double2 v = t1.sums();
+        a[0] = v.x;
+        b[0] = v.y;
+      }
     }
-    const int64_t slot = n.ptr ? 2 * t + i : t;
+    const int64_t slot = n.ptr ? 2 * t + i : int64_t(blockIdx.z) * n.tiles + t;
+    const bool any = p.r0 < p.r1;
 #pragma unroll
     for (int j = 0; j < S; ++j) {
       double2 v = {a[j], b[j]};
-      if (here) v = sum_rows(v, n.cols, red);
-      if (tr == 0 && col < vecs) n.part[slot * (BWD ? n.channels : vecs) + col * S + j] = v;
+      if (any) v = sum_rows(v, n.cols, red);
+      if (tr == 0 && on) n.part[slot * (BWD ? n.channels : vecs) + col * S + j] = v;
     }
   }
 }
@@ -707,7 +743,7 @@ __global__ void __launch_bounds__(kJoinThreads) k_join(const Norm n, int64_t job
   }
   const int vecs = n.channels / V, per = n.channels / n.groups;
   const int width = BWD ? n.channels : vecs, each = BWD ? per : vecs / n.groups;
-  const int64_t job = blockIdx.x, s = job / n.groups;
+  const uint32_t job = blockIdx.x, s = job / uint32_t(n.groups);
   const int g = int(job - s * n.groups);
   int64_t r0, r1, first, count;
   segment_rows(n, s, r0, r1);
@@ -721,8 +757,8 @@ __global__ void __launch_bounds__(kJoinThreads) k_join(const Norm n, int64_t job
   }
   double2 v = {0.0, 0.0};
 #pragma unroll 4
-  for (int64_t i = threadIdx.x; i < count * each; i += kJoinThreads) {
-    const int64_t k = i / each;
+  for (uint32_t i = threadIdx.x; i < uint32_t(count * each); i += kJoinThreads) {
+    const uint32_t k = i / uint32_t(each);
     const int c = int(i - k * each) + g * each;
     int64_t slot = first + k;
     // ragged: the second slot where the segment starts inside the tile
@@ -748,17 +784,17 @@ __global__ void __launch_bounds__(kJoinThreads) k_join(const Norm n, int64_t job
 template <typename T, int V, bool BWD, int ACT>
 __global__ void __launch_bounds__(kTileThreads) k_apply(const Norm n) {
   using P = Pack<T, V>;
+  constexpr int R = 2;  // rows in flight
   const int vecs = n.channels / V, gv = vecs / n.groups;
-  const int c = threadIdx.x % n.cols, tr = threadIdx.x / n.cols, rows = kTileThreads / n.cols;
+  const int c = threadIdx.x & (n.cols - 1), tr = threadIdx.x >> n.cols2, rows = kTileThreads >> n.cols2;
   const int col = blockIdx.y * n.cols + c;
+  const bool on = col < vecs;
   const int64_t t = blockIdx.x;
-  Piece p[2];
-  const int found = pieces_of(n, t, p);
-  if (col >= vecs) return;
-  constexpr int R = 4;  // rows in flight
-  for (int i = 0; i < found; ++i) {
-    if (p[i].seg < 0) continue;
-    const int64_t job = p[i].seg * n.groups + col / gv;
+#pragma unroll 1
+  for (int i = 0; i < (n.ptr ? 2 : 1); ++i) {
+    const Piece p = piece_of(n, t, i);
+    if (!on || p.r0 >= p.r1) continue;
+    const int64_t job = p.seg * n.groups + col / gv;
     Columns<T, V, ACT> k;
     k.set(n, col, n.stats[2 * job], n.stats[2 * job + 1]);
     float ra = 0.f, rb = 0.f;
@@ -766,45 +802,46 @@ __global__ void __launch_bounds__(kTileThreads) k_apply(const Norm n) {
       ra = float(n.mom[job].x * k.rstd);
       rb = float(n.mom[job].y * k.rstd);
     }
-    const T* px = row_in<T>(n, n.x, p[i].seg, p[i].r0 + tr) + col * V;
-    const int64_t at = (p[i].r0 + tr) * n.channels + col * V;
+    const T* px = row_in<T>(n, n.x, p.seg, p.r0 + tr) + col * V;
+    const int64_t at = (p.r0 + tr) * n.channels + col * V;
     const T* pd = static_cast<const T*>(n.dy) + at;
     T* po = static_cast<T*>(n.out) + at;
     const int64_t xs = rows * n.row_stride, ds = int64_t(rows) * n.channels;
-    int64_t left = p[i].r1 - p[i].r0 - tr;
-    auto take = [&](auto number) {  // that many rows, all of them read first
-      constexpr int N = decltype(number)::value;
-      Raw<T, V> x[N], dy[N];
+#pragma unroll 1
+    for (int left = int(p.r1 - p.r0) - tr; left > 0; left -= R * rows) {
+      Raw<T, V> x[R], dy[R];
 #pragma unroll
-      for (int u = 0; u < N; ++u) {
-        x[u].read(px + u * xs);
-        if (BWD) dy[u].read(pd + u * ds);
+      for (int u = 0; u < R; ++u) {
+        x[u] = dy[u] = Raw<T, V>{};
+        if (u * rows < left) {
+          x[u].read(px + u * xs);
+          if (BWD) dy[u].read(pd + u * ds);
+        }
       }
 #pragma unroll
-      for (int u = 0; u < N; ++u) {
-        P* out = reinterpret_cast<P*>(po + u * ds);
+      for (int u = 0; u < R; ++u) {
+        P o;
         if (BWD) {
           float dz[V], xh[V];
           k.slope(n, x[u], dy[u], dz, xh);
-          *out = k.backward(dz, xh, ra, rb);
+          o = k.backward(dz, xh, ra, rb);
         } else {
-          *out = k.forward(n, x[u]);
+          o = k.forward(n, x[u]);
         }
+        if (u * rows < left) *reinterpret_cast<P*>(po + u * ds) = o;
       }
-      px += N * xs;
-      pd += N * ds;
-      po += N * ds;
-      left -= N * rows;
-    };
-    while (left > (R - 1) * rows) take(std::integral_constant<int, R>{});
-    while (left > 0) take(std::integral_constant<int, 1>{});
+      px += R * xs;
+      pd += R * ds;
+      po += R * ds;
+    }
   }
-  if (n.ptr) {  // the rows of no segment
+  if (n.ptr && on) {  // the rows of no segment
     const int64_t a = t * n.tile, e = a + n.tile < n.length ? a + n.tile : n.length;
     const int64_t first = ptr_at(n, 0), last = ptr_at(n, n.segments);
-    for (int64_t r = a + tr; r < e; r += rows)
-      if (r < first || r >= last)
-        *reinterpret_cast<P*>(static_cast<T*>(n.out) + r * n.channels + col * V) = P{};
+    if (a < first || e > last)
+      for (int64_t r = a + tr; r < e; r += rows)
+        if (r < first || r >= last)
+          *reinterpret_cast<P*>(static_cast<T*>(n.out) + r * n.channels + col * V) = P{};
   }
 }
 
@@ -891,6 +928,7 @@ gfd_status launch(Norm n, const Cut& c, hipStream_t stream) {
   const int gv = vecs / n.groups;
   if (!n.ptr && n.length == 1 && gv <= kWave && (gv & (gv - 1)) == 0) {
     n.cols = pow2_up(vecs < kWave ? vecs : kWave);
+    n.cols2 = __builtin_ctz(n.cols);
     const int rows = kRowThreads / n.cols;
     const int64_t need = (n.segments + rows - 1) / rows, most = BWD ? c.teams : kRowBlocks;
     team_blocks = need < most ? need : most;
@@ -905,6 +943,8 @@ gfd_status launch(Norm n, const Cut& c, hipStream_t stream) {
     const int64_t mean = n.ptr ? (n.length + n.segments - 1) / n.segments : n.length;
     const int most = block / n.cols, want = pow2_up(mean < most ? (mean < 1 ? 1 : mean) : most);
     n.rows = want < most ? want : most;
+    n.cols2 = __builtin_ctz(n.cols);
+    n.rows2 = __builtin_ctz(n.rows);
     const int teams = block / (n.cols * n.rows);
     int64_t grid = (n.segments + teams - 1) / teams;
     grid = grid < c.teams ? grid : c.teams;
@@ -918,8 +958,10 @@ gfd_status launch(Norm n, const Cut& c, hipStream_t stream) {
   }
   if (c.tiled && c.slots > 0) {
     n.cols = pow2_up(vecs < kTileThreads ? vecs : kTileThreads);
-    const int64_t tiles = n.ptr ? c.tiles : n.segments * c.tiles;
-    const dim3 grid(unsigned(tiles), unsigned((vecs + n.cols - 1) / n.cols));
+    n.cols2 = __builtin_ctz(n.cols);
+    // (dense segments are fewer than kTeamBlocks here)
+    const dim3 grid(unsigned(c.tiles), unsigned((vecs + n.cols - 1) / n.cols),
+                    n.ptr ? 1u : unsigned(n.segments));
     k_sums<T, V, BWD, BWD ? ACT : GFD_ACT_NONE><<<grid, kTileThreads, 0, stream>>>(n);
     GFD_LAUNCH_CHECK();
     const int64_t jobs = n.segments * n.groups;
@@ -951,10 +993,9 @@ gfd_status check(const void* x, int dtype, int64_t segments, int64_t length, int
   return GFD_OK;
 }
 
-// tiles and slots are counted in 32 bits by the grid
-bool grid_ok(const Cut& c, int64_t segments, bool ragged) {
-  const int64_t tiles = ragged ? c.tiles : c.tiled ? segments * c.tiles : 0;
-  return tiles < (int64_t(1) << 31);
+// tiles, and the sums that k_join adds for a group, are counted in 32 bits
+bool grid_ok(const Cut& c, int channels) {
+  return !c.tiled || c.tiles < (int64_t(1) << 31) / channels;
 }
 
 }  // namespace
@@ -984,7 +1025,7 @@ gfd_status gfd_group_norm_fwd(const void* x, int dtype, int64_t segments, int64_
   if (length == 0 || (!ptr && segments == 0)) return GFD_OK;
   if (!x || !y || !aligned_to(y, dtype_size(dtype))) return GFD_ERR_ARGUMENT;
   const Cut c = cut_of(segments, length, ptr != nullptr);
-  if (!grid_ok(c, segments, ptr != nullptr)) return GFD_ERR_UNSUPPORTED;
+  if (!grid_ok(c, channels)) return GFD_ERR_UNSUPPORTED;
   Carve cv(ws, ws_bytes);
   Norm n = {};
   if (c.slots > 0 || c.tiled) {
@@ -1055,7 +1096,7 @@ gfd_status gfd_group_norm_bwd(const void* x, int dtype, int64_t segments, int64_
     });
   }
   const Cut c = cut_of(segments, length, ptr != nullptr);
-  if (!grid_ok(c, segments, ptr != nullptr)) return GFD_ERR_UNSUPPORTED;
+  if (!grid_ok(c, channels)) return GFD_ERR_UNSUPPORTED;
   Carve cv(ws, ws_bytes);
   Norm n = {};
   n.part = cv.take<double2>(size_t(c.slots + c.teams) * channels);
