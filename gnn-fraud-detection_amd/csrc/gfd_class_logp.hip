@@ -151,8 +151,11 @@ struct Top {
     const uint32_t u = v == v ? (b & 0x80000000u ? ~b : b | 0x80000000u) : 0u;
     uint32_t low = 0;
 #pragma unroll 1
-    for (uint32_t bit = 1u << 31; bit >= 1u << 16; bit >>= 1)
-      if (__popcll(__ballot(u >= (low | bit))) >= top) low |= bit;
+    for (uint32_t bit = 1u << 31; bit >= 1u << 16; bit >>= 1) {
+      const int many = __popcll(__ballot(u >= (low | bit)));
+      if (many >= top) low |= bit;
+      if (many == top) break;
+    }
     if (low < 0x00800000u) return -kInf;  // -inf, or what would be a NaN's bits
     return __uint_as_float(low & 0x80000000u ? low & 0x7FFFFFFFu : ~low);
   }

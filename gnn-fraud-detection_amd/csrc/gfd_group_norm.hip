@@ -41,7 +41,8 @@ struct Norm {
   const void* w;
   const void* b;
   double* stats;   // [segments, groups, 2]
-  double2* part;   // column sums
+  double2* part;   // forward: column sums of x and x^2
+  float2* grad_part;  // backward: of dz and dz xhat
   double2* mom;    // backward: A, B of a segment and group
   void* dw;        // backward, nullable
   void* db;
@@ -298,8 +299,7 @@ struct Shifted {
 // short segments: a team of cols x rows threads each
 // ---------------------------------------------------------------------------
 template <typename T, int V, int NC, bool BWD, int ACT>
-__global__ void __launch_bounds__(kMaxTeam) k_team(const Norm n) {
-  extern __shared__ double2 lds[];
+__device__ __forceinline__ void do_team(const Norm& n, uint32_t block, uint32_t blocks, double2* lds) {
   double2* red = lds;                   // [blockDim]
   double2* col_sum = lds + blockDim.x;  // [teams][vecs]
   using P = Pack<T, V>;
@@ -307,7 +307,7 @@ __global__ void __launch_bounds__(kMaxTeam) k_team(const Norm n) {
   const int size2 = n.cols2 + n.rows2, teams = blockDim.x >> size2;
   const int c = threadIdx.x & (n.cols - 1), tr = threadIdx.x >> n.cols2 & (n.rows - 1), team = threadIdx.x >> size2;
   double dw[NC][V] = {}, db[NC][V] = {};
-  for (int64_t s0 = int64_t(blockIdx.x) * teams; s0 < n.segments; s0 += int64_t(gridDim.x) * teams) {
+  for (int64_t s0 = int64_t(block) * teams; s0 < n.segments; s0 += int64_t(blocks) * teams) {
     auto rows_of = [&](int64_t s, int64_t& r0, int64_t& r1) {
       r0 = r1 = 0;
       if (s < n.segments) {
@@ -452,17 +452,23 @@ __global__ void __launch_bounds__(kMaxTeam) k_team(const Norm n) {
     __syncthreads();
   }
   if (BWD) {  // this block's column sums of dz and dz xhat
-    double2* part = n.part + int64_t(n.part0 + blockIdx.x) * n.channels;
+    float2* part = n.grad_part + (int64_t(n.part0) + block) * n.channels;
 #pragma unroll
     for (int k = 0; k < NC; ++k) {
       const int col = c + k * n.cols;
 #pragma unroll
       for (int j = 0; j < V; ++j) {
         const double2 v = sum_rows({db[k][j], dw[k][j]}, n.cols, red);
-        if (threadIdx.x < n.cols && col < vecs) part[col * V + j] = v;
+        if (threadIdx.x < n.cols && col < vecs) part[col * V + j] = {float(v.x), float(v.y)};
       }
     }
   }
+}
+
+template <typename T, int V, int NC, bool BWD, int ACT>
+__global__ void __launch_bounds__(kMaxTeam) k_team(const Norm n) {
+  extern __shared__ double2 lds[];
+  do_team<T, V, NC, BWD, ACT>(n, blockIdx.x, gridDim.x, lds);
 }
 
 // ---------------------------------------------------------------------------
@@ -591,11 +597,11 @@ __global__ void __launch_bounds__(kRowThreads) k_rows(const Norm n) {
     }
   }
   if (BWD) {
-    double2* part = n.part + int64_t(blockIdx.x) * n.channels;
+    float2* part = n.grad_part + int64_t(blockIdx.x) * n.channels;
 #pragma unroll
     for (int j = 0; j < V; ++j) {
       const double2 v = sum_rows({db[j], dw[j]}, n.cols, red);
-      if (threadIdx.x < n.cols && on) part[col * V + j] = v;
+      if (threadIdx.x < n.cols && on) part[col * V + j] = {float(v.x), float(v.y)};
     }
   }
 }
@@ -610,15 +616,13 @@ constexpr int kTileThreads = 256;
 // first wave of a CU waits about 0.1 us for every 64 bytes of its instructions, which for a few
 // MB of rows is most of the time.)
 template <typename T, int V, bool BWD, int ACT>
-__global__ void __launch_bounds__(kTileThreads) k_sums(const Norm n) {
+__device__ __forceinline__ void do_sums(const Norm& n, int64_t t, double2* red) {
   constexpr int S = BWD ? V : 1;
   constexpr int R = BWD ? 2 : 8;  // rows in flight
-  __shared__ double2 red[kTileThreads];
   const int vecs = n.channels / V, gv = vecs / n.groups;
   const int c = threadIdx.x & (n.cols - 1), tr = threadIdx.x >> n.cols2, rows = kTileThreads >> n.cols2;
   const int col = blockIdx.y * n.cols + c;
   const bool on = col < vecs;
-  const int64_t t = blockIdx.x;
 #pragma unroll 1
   for (int i = 0; i < (n.ptr ? 2 : 1); ++i) {
     const Piece p = piece_of(n, t, i);
@@ -699,9 +703,29 @@ __global__ void __launch_bounds__(kTileThreads) k_sums(const Norm n) {
     for (int j = 0; j < S; ++j) {
       double2 v = {a[j], b[j]};
       if (any) v = sum_rows(v, n.cols, red);
-      if (tr == 0 && on) n.part[slot * (BWD ? n.channels : vecs) + col * S + j] = v;
+      if (tr == 0 && on) {
+        if (BWD) n.grad_part[slot * n.channels + col * V + j] = {float(v.x), float(v.y)};
+        else n.part[slot * vecs + col] = v;
+      }
     }
   }
+}
+
+template <typename T, int V, bool BWD, int ACT>
+__global__ void __launch_bounds__(kTileThreads) k_sums(const Norm n) {
+  __shared__ double2 red[kTileThreads];
+  do_sums<T, V, BWD, ACT>(n, blockIdx.x, red);
+}
+
+// both, of a ragged batch: the short segments in the first ``teams`` blocks, the tiles' sums in
+// those behind them (one after the other they take 10 us longer, forward, and 14 us, backward)
+template <typename T, int V, bool BWD, int ACT>
+__global__ void __launch_bounds__(kTileThreads) k_team_sums(const Norm team, const Norm tile, uint32_t teams) {
+  extern __shared__ double2 lds[];
+  if (blockIdx.x < teams)
+    do_team<T, V, 1, BWD, ACT>(team, blockIdx.x, teams, lds);
+  else
+    do_sums<T, V, BWD, ACT>(tile, blockIdx.x - teams, lds);
 }
 
 constexpr int kJoinThreads = 256;
@@ -712,11 +736,11 @@ __device__ void join_columns(const Norm& n, int64_t slots, int c0, double2* red)
   const int c = c0 + (threadIdx.x & 3);
   double2 s = {0.0, 0.0};
   if (c < n.channels) {
-#pragma unroll 4
+#pragma unroll 8
     for (int64_t i = threadIdx.x >> 2; i < slots; i += kJoinThreads / 4) {
-      const double2 v = n.part[i * n.channels + c];
-      s.x += v.x;
-      s.y += v.y;
+      const float2 v = n.grad_part[i * n.channels + c];
+      s.x += double(v.x);
+      s.y += double(v.y);
     }
   }
   s = sum_rows(s, 4, red);
@@ -756,17 +780,27 @@ __global__ void __launch_bounds__(kJoinThreads) k_join(const Norm n, int64_t job
     count = n.tiles;
   }
   double2 v = {0.0, 0.0};
-#pragma unroll 4
-  for (uint32_t i = threadIdx.x; i < uint32_t(count * each); i += kJoinThreads) {
-    const uint32_t k = i / uint32_t(each);
-    const int c = int(i - k * each) + g * each;
-    int64_t slot = first + k;
-    // ragged: the second slot where the segment starts inside the tile
-    if (n.ptr) slot = 2 * slot + (r0 > slot * n.tile ? 1 : 0);
-    const double2 q = n.part[slot * width + c];
-    const double w = BWD ? double(affine_at<T>(n.w, n.w_f32, c, 1.f)) : 1.0;
-    v.x += w * q.x;
-    v.y += w * q.y;
+  // threads over the group's columns (a power of two of them), the others over the tiles
+  int wide2 = 0;
+  while ((1 << wide2) < each && (1 << wide2) < kJoinThreads) ++wide2;
+  const int step = kJoinThreads >> wide2;
+  // ragged: the second slot where the segment starts inside the tile
+  using Part = std::conditional_t<BWD, float2, double2>;
+  const Part* from = (BWD ? reinterpret_cast<const Part*>(n.grad_part) : reinterpret_cast<const Part*>(n.part)) +
+                     (n.ptr ? 2 * first : first) * width + g * each;
+  const int64_t pitch = n.ptr ? 2 * width : width;
+  const bool inside = n.ptr && r0 > first * n.tile;
+  for (int c = threadIdx.x & ((1 << wide2) - 1); c < each; c += 1 << wide2) {
+    const double w = BWD ? double(affine_at<T>(n.w, n.w_f32, g * each + c, 1.f)) : 1.0;
+    double2 s = {0.0, 0.0};
+#pragma unroll 8
+    for (int k = threadIdx.x >> wide2; k < int(count); k += step) {
+      const Part q = from[k * pitch + (k == 0 && inside ? width : 0) + c];
+      s.x += double(q.x);
+      s.y += double(q.y);
+    }
+    v.x += w * s.x;
+    v.y += w * s.y;
   }
   v = sum_rows(v, 1, red);
   if (threadIdx.x == 0) {
@@ -866,8 +900,8 @@ struct Cut {
 Cut cut_of(int64_t segments, int64_t length, bool ragged) {
   Cut c;
   const int64_t rows = ragged ? length : segments * length;
-  // tiles: about 2048 of them, 32 to 512 rows
-  int64_t tile = pow2_up((rows + 2047) / 2048);
+  // tiles: about 1024 of them, 32 to 512 rows
+  int64_t tile = pow2_up((rows + 1023) / 1024);
   tile = tile < 32 ? 32 : tile > 512 ? 512 : tile;
   c.tile = int(tile);
   if (ragged) {
@@ -925,6 +959,7 @@ template <typename T, int V, bool BWD, int ACT>
 gfd_status launch(Norm n, const Cut& c, hipStream_t stream) {
   const int vecs = n.channels / V;
   int64_t team_blocks = 0;
+  bool summed = false;  // the tiles' sums
   const int gv = vecs / n.groups;
   if (!n.ptr && n.length == 1 && gv <= kWave && (gv & (gv - 1)) == 0) {
     n.cols = pow2_up(vecs < kWave ? vecs : kWave);
@@ -950,10 +985,17 @@ gfd_status launch(Norm n, const Cut& c, hipStream_t stream) {
     grid = grid < c.teams ? grid : c.teams;
     team_blocks = grid;
     const size_t lds = sizeof(double2) * (size_t(block) + size_t(teams) * vecs);
-    if (nc == 1)
+    if (c.tiled && block == kTileThreads && grid + c.tiles < (int64_t(1) << 31)) {
+      Norm m = n;
+      m.cols = pow2_up(vecs);
+      m.cols2 = __builtin_ctz(m.cols);
+      k_team_sums<T, V, BWD, ACT><<<unsigned(grid + c.tiles), block, lds, stream>>>(n, m, unsigned(grid));
+      summed = true;
+    } else if (nc == 1) {
       k_team<T, V, 1, BWD, ACT><<<int(grid), block, lds, stream>>>(n);
-    else if constexpr (V == 1)  // more vectors than threads
+    } else if constexpr (V == 1) {  // more vectors than threads
       k_team<T, V, 2, BWD, ACT><<<int(grid), block, lds, stream>>>(n);
+    }
     GFD_LAUNCH_CHECK();
   }
   if (c.tiled && c.slots > 0) {
@@ -962,7 +1004,7 @@ gfd_status launch(Norm n, const Cut& c, hipStream_t stream) {
     // (dense segments are fewer than kTeamBlocks here)
     const dim3 grid(unsigned(c.tiles), unsigned((vecs + n.cols - 1) / n.cols),
                     n.ptr ? 1u : unsigned(n.segments));
-    k_sums<T, V, BWD, BWD ? ACT : GFD_ACT_NONE><<<grid, kTileThreads, 0, stream>>>(n);
+    if (!summed) k_sums<T, V, BWD, BWD ? ACT : GFD_ACT_NONE><<<grid, kTileThreads, 0, stream>>>(n);
     GFD_LAUNCH_CHECK();
     const int64_t jobs = n.segments * n.groups;
     const int64_t columns = BWD && (n.dw || n.db) ? (n.channels + 3) / 4 : 0;
@@ -1008,7 +1050,8 @@ size_t gfd_group_norm_workspace_size(int64_t segments, int64_t length, int ragge
   if (!ragged && (segments == 0 || length == 0)) return 0;
   const Cut c = cut_of(segments, length, ragged != 0);
   Sizer z;
-  z.take<double2>(size_t(c.slots + (backward ? c.teams : 0)) * channels);
+  if (backward) z.take<float2>(size_t(c.slots + c.teams) * channels);
+  else z.take<double2>(size_t(c.slots) * channels);
   z.take<double2>(c.tiled ? size_t(segments) * groups : 0);
   return z.off;
 }
@@ -1099,7 +1142,7 @@ gfd_status gfd_group_norm_bwd(const void* x, int dtype, int64_t segments, int64_
   if (!grid_ok(c, channels)) return GFD_ERR_UNSUPPORTED;
   Carve cv(ws, ws_bytes);
   Norm n = {};
-  n.part = cv.take<double2>(size_t(c.slots + c.teams) * channels);
+  n.grad_part = cv.take<float2>(size_t(c.slots + c.teams) * channels);
   n.mom = cv.take<double2>(c.tiled ? size_t(segments) * groups : 0);
   if (!cv.ok) return GFD_ERR_WORKSPACE;
   n.x = x;
