@@ -19,7 +19,8 @@
 //     their lists' last entries.
 // Rows of up to kNarrow classes are read by teams of 1 to 32 lanes, longer ones
 // by a wave, long ones by a block; few long rows are split over blocks whose
-// partial results a second kernel joins.
+// partial results a second kernel joins.  2048 rows of 203769 bf16 logits: 153 us
+// without a list (5.4 TB/s), 225 us with the best 8; backward 322 us.
 #include "gfd_rowops.h"
 
 using namespace gfd;
@@ -28,11 +29,16 @@ namespace {
 
 constexpr int kThreads = 256;
 constexpr int kWaves = kThreads / kWave;
-constexpr int kNarrow = 128;       // classes of the team kernel: 32 lanes of 4
-constexpr int kWaveRow = 4096;     // classes a single wave reads
+// classes of the team kernel: 32 lanes of 4 (100000 rows of 128 in bf16, no list and the best 5:
+// 16 and 59 us, by a wave each 37 and 106; of 256 in teams of 64 lanes 38 and 124, by a wave 38
+// and 104)
+constexpr int kNarrow = 128;
 constexpr int kMaxTop = 64;        // a list entry a lane
-constexpr int kMinSplit = 4096;    // classes of a split, at least
-constexpr int kFill = 1024;        // blocks that fill the card: rows are split below it
+// classes of a split, at least (a row of 16384, the best 8: 17.5 us, of splits of 16384 19.4; a
+// row of 1000000: 33 us, of splits of 2048 42)
+constexpr int kMinSplit = 4096;
+// rows are split below it (900 rows of 65536, the best 8: 56 us whole, 63 us in two)
+constexpr int kFill = 512;
 constexpr float kSlack = 8.f;
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kInf = __builtin_inff();
@@ -547,9 +553,19 @@ __global__ void __launch_bounds__(kWave) k_fwd_join(const T* __restrict__ x, int
   }
 }
 
+// A row by one wave, or by a block's: a wave where the rows fill the card, which costs no joins
+// (2000 rows of 4096, the best 5: 19 us, by blocks 22; 20000 rows: 68 and 132), a block where
+// they do not (256 rows: 17 and 12 us).  Longer rows read the same by either, but a list a wave
+// is four lists a row (20000 rows of 16384, the best 5: 148 and 239 us; 4096 rows of 65536: 119
+// and 123; no list: 116 and 109).
+inline bool by_wave(int64_t rows, int64_t classes, int top) {
+  return classes <= 1024 || (rows >= 1024 && classes <= 4096) ||
+         (top > 0 && rows >= 4096 && classes <= 65536);
+}
+
 // how many blocks share a row, and the classes of one (a multiple of 16)
-inline int splits_of(int64_t rows, int64_t classes) {
-  if (classes <= kWaveRow || rows >= kFill) return 1;
+inline int splits_of(int64_t rows, int64_t classes, int top) {
+  if (by_wave(rows, classes, top) || rows >= kFill) return 1;
   const int64_t by_rows = (kFill + rows - 1) / rows;
   const int64_t by_classes = (classes + kMinSplit - 1) / kMinSplit;
   return int(by_rows < by_classes ? by_rows : by_classes);
@@ -689,7 +705,7 @@ extern "C" {
 
 size_t gfd_class_logp_workspace_size(int64_t rows, int64_t classes, int top) {
   if (bad_shape(rows, classes, 0, top) || rows == 0) return 0;
-  const int s = splits_of(rows, classes);
+  const int s = splits_of(rows, classes, top);
   if (s == 1) return 0;
   Sizer z;
   z.take<Partial>(size_t(rows) * s);
@@ -710,7 +726,7 @@ gfd_status gfd_class_logp_fwd(const void* logits, int dtype, int64_t rows, int64
   if (!aligned_to(logits, dtype_size(dtype))) return GFD_ERR_ARGUMENT;
   const RowOut o{target, ignore_index, logp, entropy, top_logp, top_class, stats};
   const int n = int(classes);
-  const int splits = splits_of(rows, classes);
+  const int splits = splits_of(rows, classes, top);
   Partial* part = nullptr;
   Entry* part_top = nullptr;
   if (splits > 1) {
@@ -736,7 +752,7 @@ gfd_status gfd_class_logp_fwd(const void* logits, int dtype, int64_t rows, int64
       narrow(std::integral_constant<int, 16>{});
     } else if (n <= kNarrow) {
       narrow(std::integral_constant<int, 32>{});
-    } else if (n <= kWaveRow) {
+    } else if (by_wave(rows, classes, top)) {
       const int64_t blocks = (rows + kWaves - 1) / kWaves;
       k_fwd_wide<T, 1, false><<<int(blocks < 65536 ? blocks : 65536), kThreads, 0, stream>>>(
           x, rows, n, row_stride, top, 1, n, nullptr, nullptr, o);
@@ -789,13 +805,17 @@ gfd_status gfd_class_logp_bwd(const void* logits, int dtype, int64_t rows, int64
     // 16-byte vectors where every row of both starts at the same place of one
     const bool same = (reinterpret_cast<uintptr_t>(x) - reinterpret_cast<uintptr_t>(g)) % 16 == 0 &&
                       (rows == 1 || (row_stride - classes) * int64_t(sizeof(T)) % 16 == 0);
+    // 16 lanes up to 512 classes: 100000 rows of 256 23 us, of 512 36 us, a wave a row 44 and 50 us
+    // (1000 rows 4.5 and 5.7 us, a wave 4.0); 256 rows of 4096: a wave a row 7.8 us, a block 4.6 us
     if (n <= 4) {
       launch(one, integral_constant<int, 1>{}, 1, n);
     } else if (n <= 16) {
       launch(one, integral_constant<int, 4>{}, 1, n);
     } else if (n <= 128) {
       launch(one, integral_constant<int, 16>{}, 1, n);
-    } else if (n <= kWaveRow) {
+    } else if (n <= 512 && same) {
+      launch(vec, integral_constant<int, 16>{}, 1, n);
+    } else if (by_wave(rows, classes, 0)) {
       if (same) launch(vec, integral_constant<int, 64>{}, 1, n);
       else launch(one, integral_constant<int, 64>{}, 1, n);
     } else {

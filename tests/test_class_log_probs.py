@@ -114,7 +114,8 @@ def test_classes(V, dtype):
 
 
 @pytest.mark.gpu
-@pytest.mark.parametrize("N,V", [(1, 1), (1, 100000), (2, 70001), (5000, 2), (3001, 7), (1500, 130), (1100, 4500)])
+@pytest.mark.parametrize("N,V", [(1, 1), (1, 100000), (2, 70001), (5000, 2), (3001, 7), (1500, 130), (1100, 4500),
+                                 (1100, 3000), (4100, 4200), (520, 6000)])
 def test_rows(N, V):
     check(logits(N, V, torch.float32), targets(N, V), min(V, 3))
 
