@@ -104,6 +104,7 @@ def c1_gat2_forward(dev, steps=20, warmup=3, cpu_runs=3):
 
 
 def c2_gat3_train_step(dev, steps=20, warmup=3, cpu_runs=3):
+    from gfd.optim import Adam
     d = _elliptic(dev)
     m = _model("gat", 165, 3, dev).train()
     opt = torch.optim.Adam(m.parameters(), lr=1e-3, weight_decay=5e-4)
@@ -111,7 +112,7 @@ def c2_gat3_train_step(dev, steps=20, warmup=3, cpu_runs=3):
     mask = d["y"] != -1
     yl = d["y"][mask].float()
 
-    def step():
+    def step(m=m, opt=opt):
         opt.zero_grad()
         logits = m(d["x"], d["edge_index"])
         loss = crit(logits[mask].squeeze(1), yl)
@@ -119,6 +120,9 @@ def c2_gat3_train_step(dev, steps=20, warmup=3, cpu_runs=3):
         opt.step()
 
     med, mean = _time(step, steps, warmup)
+    m2 = _model("gat", 165, 3, dev).train()        # the same step, the library's optimizer
+    opt2 = Adam(m2.parameters(), lr=1e-3, weight_decay=5e-4)
+    med2, _ = _time(lambda: step(m2, opt2), steps, warmup)
     fwd_med, _ = _time(lambda: m(d["x"], d["edge_index"]), steps, warmup)
     # CPU baseline: the same step with the oracle's PyG-dataflow model on the
     # host (train.py:105-143's loop body), same weights, 1 warm-up + median
@@ -141,7 +145,7 @@ def c2_gat3_train_step(dev, steps=20, warmup=3, cpu_runs=3):
     return {"workload": f"GAT 3 layers train step (fwd + BCE(pos_weight 50) + bwd + Adam), "
                         f"Elliptic-shaped N={d['N']} E={d['E']} F=165, dropout 0.2",
             "unit": "edges/s", "value": d["E"] / (med * 1e-3), "ms_per_step": med,
-            "ms_mean": mean, "forward_ms_train_mode": fwd_med,
+            "ms_mean": mean, "ms_per_step_gfd_adam": med2, "forward_ms_train_mode": fwd_med,
             "cpu_baseline": {"value": d["E"] / tt[len(tt) // 2], "unit": "edges/s",
                              "median_s": tt[len(tt) // 2], "min_s": tt[0], "runs": cpu_runs,
                              "cores": torch.get_num_threads(), "kind": "port",

@@ -22,6 +22,7 @@ train.py:143): the same constructor arguments and update, over
 """
 from __future__ import annotations
 
+from collections import defaultdict
 from operator import attrgetter
 from typing import Dict, Tuple
 
@@ -55,7 +56,8 @@ class Adam(torch.optim.Optimizer):
                  weight_decay: float = 0.0, *, state_bits: int = 32, seed: int = 0):
         self._flat: Dict[int, dict] = {}
         super().__init__(params, dict(lr=lr, betas=tuple(betas), eps=eps,
-                                      weight_decay=weight_decay, state_bits=state_bits, seed=seed))
+                                      weight_decay=weight_decay, state_bits=state_bits, seed=seed,
+                                      decoupled_weight_decay=self._decoupled))
 
     def add_param_group(self, param_group: dict) -> None:
         super().add_param_group(param_group)
@@ -65,8 +67,7 @@ class Adam(torch.optim.Optimizer):
             self.param_groups.pop()
             raise
 
-    @staticmethod
-    def _check_group(group: dict) -> None:
+    def _check_group(self, group: dict) -> None:
         lr, (b1, b2) = group["lr"], group["betas"]
         if isinstance(lr, torch.Tensor):
             if lr.dim() != 0 or lr.dtype != torch.float32:
@@ -86,6 +87,9 @@ class Adam(torch.optim.Optimizer):
         for other in ("amsgrad", "maximize"):
             if group.get(other):
                 raise NotImplementedError(f"gfd Adam: {other} is not supported")
+        if group["decoupled_weight_decay"] != self._decoupled:
+            raise ValueError("gfd Adam: Adam adds the weight decay to the gradient, AdamW applies it to "
+                             "the parameter; a group is of the other kind")
         for p in group["params"]:
             if p.dtype not in _CODES:
                 raise TypeError("gfd Adam: parameters must be float32, bfloat16 or float16 "
@@ -164,15 +168,23 @@ class Adam(torch.optim.Optimizer):
 
     @torch.no_grad()
     def load_state_dict(self, state_dict: dict) -> None:
-        """Of this class, or of torch.optim.Adam / AdamW (fp32 states)."""
+        """Of this class, or of torch.optim.Adam / AdamW (fp32 states).  One that is refused leaves
+        the optimizer as it was."""
         groups = []
         for g, mine in zip(state_dict["param_groups"], self.param_groups):
-            groups.append({**{k: mine[k] for k in ("state_bits", "seed")}, **g})
+            groups.append({**{k: mine[k] for k in ("state_bits", "seed", "decoupled_weight_decay")}, **g})
         if len(groups) != len(state_dict["param_groups"]):
             raise ValueError("loaded state dict has a different number of parameter groups")
-        super().load_state_dict({"state": {}, "param_groups": groups})
-        self._flat.clear()
-        self.state.clear()
+        before = self._flat, self.state, self.param_groups
+        try:
+            super().load_state_dict({"state": {}, "param_groups": groups})
+            self._flat, self.state = {}, defaultdict(dict)
+            self._fill_groups(groups, state_dict)
+        except Exception:
+            self._flat, self.state, self.param_groups = before
+            raise
+
+    def _fill_groups(self, groups: list, state_dict: dict) -> None:
         for gi, (group, saved) in enumerate(zip(self.param_groups, groups)):
             self._check_group(group)
             if not any(k in state_dict["state"] for k in saved["params"]):

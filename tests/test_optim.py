@@ -326,6 +326,38 @@ def test_loads_torch_states():
         Adam([{"params": [p]}, {"params": make([3], torch.float32)}]).load_state_dict(eight.state_dict())
 
 
+def test_other_kind_of_decay_is_not_loaded():
+    """A state dict of AdamW into Adam, or the other way, would train on with another rule."""
+    from gfd.optim import Adam, AdamW
+    p = torch.zeros(4, requires_grad=True)
+    for ours, theirs in ((Adam([p], weight_decay=0.1), AdamW([p], weight_decay=0.1)),
+                         (AdamW([p]), Adam([p])), (Adam([p]), torch.optim.AdamW([p]))):
+        with pytest.raises(ValueError, match="of the other kind"):
+            ours.load_state_dict(theirs.state_dict())
+        assert ours.param_groups[0]["lr"] == 1e-3
+    AdamW([p]).load_state_dict(torch.optim.AdamW([p]).state_dict())
+
+
+@pytest.mark.gpu
+def test_a_refused_state_dict_changes_nothing():
+    from gfd.optim import Adam
+    p, q = make([300, (7, 5)], torch.float32)
+    opt, same = Adam([p, q], lr=0.1), Adam([r.detach().clone().requires_grad_() for r in (p, q)], lr=0.1)
+    for r, s in zip(same.param_groups[0]["params"], (p, q)):
+        r.grad = s.grad.clone()
+    opt.step()
+    same.step()
+    bad = copy.deepcopy(opt.state_dict())
+    bad["state"][1]["exp_avg"] = torch.zeros(3)
+    bad["param_groups"][0]["lr"] = 7.0
+    with pytest.raises(ValueError, match="exp_avg"):
+        opt.load_state_dict(bad)
+    opt.step()
+    same.step()
+    for r, s in zip(same.param_groups[0]["params"], (p, q)):
+        assert torch.equal(r, s) and torch.equal(same.state[r]["exp_avg"], opt.state[s]["exp_avg"])
+
+
 @pytest.mark.gpu
 def test_eight_bits_round_without_bias():
     """65536 elements with one moment between two codes: their mean is the moment's, within six
