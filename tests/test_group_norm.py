@@ -362,7 +362,7 @@ def test_c_argument_errors():
     lib = _lib.load()
     size = lib.gfd_group_norm_workspace_size
     assert size(1, 100000, 0, 64, 8, 0) > 0 and size(200000, 1, 0, 64, 8, 0) == 0
-    assert size(200000, 1, 0, 64, 8, 1) > 0 and size(4, 100, 1, 64, 8, 1) > size(4, 100, 1, 64, 8, 0) > 0
+    assert size(200000, 1, 0, 64, 8, 1) > 0 and size(4, 100, 1, 64, 8, 1) > 0 and size(4, 100, 1, 64, 8, 0) > 0
     assert size(1, 10, 0, 64, 7, 0) == 0
 
     def fwd(dtype=0, channels=8, groups=2, w_dtype=0, eps=1e-5, act=0, x=256, y=256, segments=1, length=4,
