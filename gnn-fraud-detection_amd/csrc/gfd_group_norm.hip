@@ -14,14 +14,15 @@
 // rounding each, beside as many roundings of dz itself.
 //   * A segment of one row (a node) is its group's lanes' own affair: they exchange
 //     their sums and keep x in registers (k_rows); the backward finds the
-//     statistics again.  203769 rows of 64 bf16 channels: forward 24 us, backward
+//     statistics again.  203769 rows of 64 fp32 channels: forward 24 us, backward
 //     30 us and 4 us for the weights (46, 59 and 12 us as teams with kept statistics).
 //   * A short segment is normalised by one team of threads (k_team): its rows
 //     are read twice, the second time from cache, in one launch.
 //   * A long one is cut into tiles of rows: k_sums writes each tile's column
 //     sums, k_join joins those of a segment and group in a fixed order, k_apply
-//     writes the result.  1048576 rows of 64 bf16 channels: forward 37 + 5 + 46 us,
-//     backward 55 + 6 + 67 us, where the bytes take 53 and 79 us at the rate of a copy.  A ragged segment is long when it has more rows than a
+//     writes the result.  8 x 16384 rows of 512 bf16 channels: forward 35 + 5 +
+//     46 us, backward 55 + 6 + 67 us; what the two passes read and write takes 79
+//     and 132 us at the rate of a copy.  A ragged segment is long when it has more rows than a
 //     tile; then it holds the first or the last row of every tile that it
 //     touches, so that a tile meets at most two of them and finds them by two
 //     binary searches, however many segments there are.

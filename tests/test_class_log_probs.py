@@ -322,6 +322,25 @@ def test_refused_without_a_device():
         GAT(5, 64, 1).log_probs(torch.zeros(2, 5), None)
 
 
+@pytest.mark.gpu
+def test_offsets_past_32_bits():
+    """The last rows of more than 2^31 logits give what they give alone."""
+    from gfd.fused import class_log_probs
+    V = 203769
+    rows = 2 ** 31 // V + 700
+    x = torch.empty((rows, V), dtype=torch.bfloat16, device=DEV).normal_()
+    t = torch.randint(V, (rows,), generator=torch.Generator().manual_seed(4)).to(DEV)
+
+    def run(x, t):
+        xr = x.detach().requires_grad_()
+        r = class_log_probs(xr, t, 4)
+        gx, = torch.autograd.grad((r.log_prob.sum(), r.entropy.sum(), r.top_log_probs[:, 1].sum()), xr)
+        return tuple(o.detach() for o in r) + (gx,)
+
+    for a, c in zip(run(x, t), run(x[-600:], t[-600:])):
+        assert torch.equal(a[-600:], c)
+
+
 def test_c_argument_errors():
     from gfd import _lib
     lib = _lib.load()

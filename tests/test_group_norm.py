@@ -299,6 +299,33 @@ def test_stream_and_graph():
 
 
 @pytest.mark.gpu
+def test_offsets_past_32_bits():
+    """The last rows of more than 2^31 elements give what they give alone: rows of their own, two
+    long segments, and short ones behind a long one."""
+    from gfd.fused import group_norm
+    rows = 2 ** 31 // 64 + 100002
+    x = torch.empty((rows, 64), dtype=torch.bfloat16, device=DEV).normal_()
+    w, b = affine(64, torch.float32)
+
+    def run(x, g, ptr=None):
+        xr = x.detach().requires_grad_()
+        y = group_norm(xr, 8, w, b, act="silu", ptr=ptr)
+        return y.detach(), torch.autograd.grad(y, xr, g)[0]
+
+    g = torch.empty_like(x).normal_()
+    for whole, last in (((x, g), slice(-1000, None)), ((x.view(2, -1, 64), g.view(2, -1, 64)), slice(1, None))):
+        for a, c in zip(run(*whole), run(*(t[last] for t in whole))):
+            assert torch.equal(a[last], c)
+    ptr = torch.tensor([0, rows - 5000, rows - 4990, rows - 2, rows], device=DEV)
+    y, gx = run(x, g, ptr)
+    tail = x[-5000:]
+    ry, size, rx, _, _, back = reference(tail, 8, w, b, 1e-5, "silu", [10, 4988, 2], g[-5000:])
+    assert ((y[-5000:].cpu().double() - ry).abs() <= OPS * size + 2.0 ** -8 * ry.abs()).all()
+    scale = 1.2 * w.abs().max().item() * g[-5000:].abs().max().item() * (1 + size.max().item())
+    assert ((gx[-5000:].cpu().double() - rx).abs() <= OPS * scale * 3 * back + 2.0 ** -8 * rx.abs()).all()
+
+
+@pytest.mark.gpu
 def test_same_result_twice():
     from gfd.fused import group_norm
     x, g = data((5000, 64), torch.bfloat16), data((5000, 64), torch.bfloat16, seed=4)

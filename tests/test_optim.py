@@ -170,6 +170,29 @@ def test_large_tensor_takes_several_rounds_of_blocks():
 
 
 @pytest.mark.gpu
+def test_offsets_past_32_bits():
+    """The last elements of a parameter of more than 2^32, and one behind it, are updated as they
+    are alone (a first step's update does not depend on how its states are rounded)."""
+    from gfd.optim import Adam
+    n = 2 ** 32 + 5003
+    p = torch.zeros(n, dtype=torch.bfloat16, device=DEV)
+    p.grad = torch.zeros_like(p)
+    q, r = make([5003, 700], torch.bfloat16)
+    p[-5003:] = q.detach()
+    p.grad[-5003:] = q.grad
+    s = r.detach().clone()
+    s.grad = r.grad.clone()
+    big = Adam([p.requires_grad_(), s.requires_grad_()], lr=0.05, state_bits=8)
+    alone = Adam([q, r], lr=0.05, state_bits=8)
+    big.step()
+    alone.step()
+    assert torch.equal(p[-5003:], q) and torch.equal(s, r) and not p[:-5003].any()
+    m, v = (big.state[p][k][-5003:].float() for k in ("exp_avg", "exp_avg_sq"))
+    assert m.ne(0).any() and v.ne(0).sum() == q.grad.ne(0).sum()
+    assert not big.state[p]["exp_avg"][:1000].float().any()
+
+
+@pytest.mark.gpu
 def test_missing_gradients_are_skipped():
     from gfd.optim import Adam
     params = make([300, 40, 500], torch.float32)
