@@ -217,6 +217,7 @@ def ptr(t) -> int | None:
 def stream_handle(device=None) -> int:
     import torch
     raw = getattr(torch._C, "_cuda_getCurrentRawStream", None)   # 2 us less than a Stream object
-    if raw is not None and device is not None and getattr(device, "index", None) is not None:
+    # (a device's name has an ``index`` too: the method of a string)
+    if raw is not None and isinstance(device, torch.device) and device.index is not None:
         return raw(device.index)
     return torch.cuda.current_stream(device).cuda_stream

@@ -237,3 +237,18 @@ def test_sharded_inference_refuses_group_norms():
     m = _model().eval()
     with torch.no_grad(), pytest.raises(NotImplementedError, match="norm='group'"):
         gdist.model_forward_sharded(m, None, None, None)
+
+
+def test_stream_of_any_form_of_a_device(monkeypatch):
+    """A device by its name, as an object with or without an index, or none at all."""
+    from gfd import _lib
+
+    class Stream:
+        cuda_stream = 7
+
+    seen = []
+    monkeypatch.setattr(torch.cuda, "current_stream", lambda device=None: seen.append(device) or Stream)
+    monkeypatch.setattr(torch._C, "_cuda_getCurrentRawStream", lambda index: 100 + int(index), raising=False)
+    for device in ("cuda", "cuda:0", torch.device("cuda"), None):
+        assert _lib.stream_handle(device) == 7 and seen.pop() == device
+    assert _lib.stream_handle(torch.device("cuda", 2)) == 102 and not seen
