@@ -599,8 +599,10 @@ gfd_status gfd_rows_copy(const float* src, int64_t src_stride, const int32_t* sr
  *           outside the rows.
  * x, y: GFD_DTYPE_F32 / BF16 / F16, channels contiguous; y (and grad_y /
  * grad_x) contiguous in the rows' order.  weight / bias [channels], nullable
- * (identity), w_dtype F32 or x's.  Statistics and sums are fp64; stats (fp64
- * [segments, groups, 2] = mean, 1/sqrt(var + eps)) is nullable in the forward
+ * (identity), w_dtype F32 or x's.  Sums are fp64, or fp32 over a few rows about
+ * one of their elements, which fp64 joins: a level far above the spread costs no
+ * digits, and deviations whose squares leave fp32 (about 1e19) are not served.
+ * stats (fp64 [segments, groups, 2] = mean, 1/sqrt(var + eps)) is nullable in the forward
  * and what the backward takes; dense segments of one row keep none (stats NULL:
  * the backward finds them again).  channels <= 2048 and a multiple of groups.
  * GELU is the erf form.  relu's side is decided in fp64 where fp32 cannot
