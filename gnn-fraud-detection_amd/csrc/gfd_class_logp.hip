@@ -125,6 +125,32 @@ __device__ __forceinline__ float above(float v) {  // the next float
 }
 __device__ __forceinline__ float below(float v) { return -above(-v); }
 
+struct Entry {  // of a list
+  float val;
+  int cls;
+};
+
+// appends the wanted entries of the lanes to those found, up to kWave
+__device__ __forceinline__ void gather(bool wanted, Entry e, Entry* found, int& count) {
+  const unsigned long long some = __ballot(wanted);
+  const int at = count + __builtin_amdgcn_mbcnt_hi(uint32_t(some >> 32),
+                                                   __builtin_amdgcn_mbcnt_lo(uint32_t(some), 0u));
+  if (wanted && at < kWave) found[at] = e;
+  count += __popcll(some);
+}
+
+// a lane's entry's place among the ``count`` of the first lanes; behind them, a place of its own
+__device__ __forceinline__ int rank_of(Entry e, int count) {
+  const int lane = threadIdx.x & 63;
+  int rank = lane < count ? 0 : lane;
+  for (int i = 0; i < count; ++i) {
+    const float v = lane_of(e.val, i);
+    const int c = __builtin_amdgcn_readlane(e.cls, i);
+    if (v > e.val || (v == e.val && c < e.cls)) ++rank;
+  }
+  return rank;
+}
+
 struct Top {
   float val = __builtin_nanf("");
   int cls = 0;
@@ -190,6 +216,8 @@ struct Top {
   // The logits x of a wave's vector, ``have`` of a lane's N from class cls0 on, those below
   // ``least`` not wanted.  They come in the order of their classes, lane by lane, and (ORDERED)
   // after all lower classes: once the list is full, one that equals its last entry is not.
+  // (Many at once by their ranks, as k_fwd_join does, is no faster: 20000 rows of 16384, the best
+  // 5: 172 us, one by one 159; a row of 203769, the best 10: 19 and 20 us.)
   template <bool ORDERED, int N>
   __device__ __forceinline__ void take(const float (&x)[N], int have, int cls0, int top, float least) {
     float best = __builtin_nanf("");
@@ -235,19 +263,31 @@ __device__ __forceinline__ float logp_of(float x, float r, float ls) {
   return r == -kInf && ls == -kInf ? -kInf : (x - r) - ls;
 }
 
+// the given class of a row and its logit
+struct Given {
+  int64_t c;
+  float x;
+  bool known;  // in the classes
+};
 template <typename T>
-__device__ __forceinline__ void write_row(const RowOut& o, int64_t row, const T* x, int64_t classes,
-                                          float r, float s, float t) {
+__device__ __forceinline__ Given given_of(const RowOut& o, int64_t row, const T* x, int64_t classes) {
+  Given g = {0, 0.f, false};
+  if (o.logp) {
+    g.c = o.target[row];
+    g.known = g.c >= 0 && g.c < classes;
+    if (g.known) g.x = to_f32(x[g.c]);
+  }
+  return g;
+}
+
+__device__ __forceinline__ void write_row(const RowOut& o, int64_t row, const Given& g, float r, float s,
+                                          float t) {
   const float ls = s == 0.f ? -kInf : logf(s);
   o.stats[2 * row] = r;
   o.stats[2 * row + 1] = ls;
   o.entropy[row] = s == 0.f ? 0.f : ls - t / s;
-  if (o.logp) {
-    const int64_t c = o.target[row];
-    o.logp[row] = c == o.ignore ? 0.f
-                  : c >= 0 && c < classes ? logp_of(to_f32(x[c]), r, ls)
-                                          : __builtin_nanf("");
-  }
+  if (o.logp)
+    o.logp[row] = g.c == o.ignore ? 0.f : g.known ? logp_of(g.x, r, ls) : __builtin_nanf("");
 }
 
 // ---------------------------------------------------------------------------
@@ -275,7 +315,7 @@ __global__ void __launch_bounds__(kThreads) k_fwd_narrow(const T* __restrict__ x
     for (int j = 0; j < 4; ++j) a.add(v[j]);
     a.s = team_sum<W>(a.s);
     a.t = team_sum<W>(a.t);
-    if (l == 0) write_row(o, row, xr, classes, a.r, a.s, a.t);
+    if (l == 0) write_row(o, row, given_of(o, row, xr, classes), a.r, a.s, a.t);
     if (top) {
       const float ls = a.s == 0.f ? -kInf : logf(a.s);
       // a taken entry, one outside of the classes and NaN are none: NaN
@@ -426,11 +466,6 @@ __device__ __forceinline__ void scan_row(const T* xr, int begin, int end, int w,
   }
 }
 
-struct Entry {  // of a list
-  float val;
-  int cls;
-};
-
 // the list of a row, a lane an entry; of a row with a NaN, some classes
 __device__ __forceinline__ void write_top(const RowOut& o, int64_t row, int top, const Top& best,
                                           float r, float s) {
@@ -498,7 +533,7 @@ __global__ void __launch_bounds__(kThreads, 8) k_fwd_wide(const T* __restrict__ 
         if (lane == 0) part[job] = {a.r, a.s, a.t};
         if (lane < top) part_top[job * top + lane] = {best.val, best.cls};
       } else {
-        if (lane == 0) write_row(o, row, xr, classes, a.r, a.s, a.t);
+        if (lane == 0) write_row(o, row, given_of(o, row, xr, classes), a.r, a.s, a.t);
         write_top(o, row, top, best, a.r, a.s);
       }
     }
@@ -506,17 +541,41 @@ __global__ void __launch_bounds__(kThreads, 8) k_fwd_wide(const T* __restrict__ 
   }
 }
 
-// a wave a row: the splits' sums and lists
+// a wave a row: the splits' sums and lists.  ``need`` lanes whose lists' entry number ``level`` is
+// not below some value have ``top`` entries that are not: a bound of the row's list.  The few
+// entries not below it are gathered, and each counts those before it (one row of 203769, the
+// best 10: 4.7 us; entries put into a list one by one 11.3 us)
 template <typename T>
 __global__ void __launch_bounds__(kWave) k_fwd_join(const T* __restrict__ x, int64_t rows,
                                                     int classes, int64_t stride, int top,
                                                     int splits, const Partial* __restrict__ part,
                                                     const Entry* __restrict__ part_top, RowOut o) {
+  __shared__ Entry found[kWave];
   const int lane = threadIdx.x;
   for (int64_t row = blockIdx.x; row < rows; row += gridDim.x) {
+    // everything it reads, before anything waits for it
+    const int n = splits * top;
+    const Entry* from = part_top + row * n;
+    const Given given = given_of(o, row, x + row * stride, classes);
+    Partial p = {-kInf, 0.f, 0.f};
+    const int lanes = splits < kWave ? splits : kWave;
+    const int level = (top - 1) / lanes, need = (top + level) / (level + 1);
+    float head = __builtin_nanf("");
+    if (lane < splits) {
+      p = part[row * splits + lane];
+      if (top) head = from[lane * top + level].val;
+    }
+    Entry e[8];
+    auto read = [&](int i0) {
+#pragma unroll
+      for (int k = 0; k < 8; ++k) {
+        e[k] = {__builtin_nanf(""), 0};
+        if (i0 + k * 64 + lane < n) e[k] = from[i0 + k * 64 + lane];
+      }
+    };
+    read(0);
     Sums a;
-    for (int i = lane; i < splits; i += 64) {
-      const Partial p = part[row * splits + i];
+    for (int i = lane; i < splits;) {
       if (p.r > a.r) a.move(p.r);
       Sums b;
       b.r = p.r;
@@ -525,30 +584,40 @@ __global__ void __launch_bounds__(kWave) k_fwd_join(const T* __restrict__ x, int
       if (p.r != -kInf) b.move(a.r);
       a.s += b.s;
       a.t += b.t;
+      if ((i += 64) < splits) {
+        p = part[row * splits + i];
+        if (top) head = max_f(head, from[i * top + level].val);
+      }
     }
     a.join();
-    if (lane == 0) write_row(o, row, x + row * stride, classes, a.r, a.s, a.t);
+    if (lane == 0) write_row(o, row, given, a.r, a.s, a.t);
     if (top) {
-      Top best;
-      const int n = splits * top;
-      const Entry* from = part_top + row * n;
-      for (int i0 = 0; i0 < n; i0 += 512) {
-        Entry e[8];
+      const float least = Top::bound_of(head, need);
+      int count = 0;  // of the entries not below it
+      for (int i0 = 0; i0 < n;) {
 #pragma unroll
-        for (int k = 0; k < 8; ++k) {
-          e[k] = {__builtin_nanf(""), 0};
-          if (i0 + k * 64 + lane < n) e[k] = from[i0 + k * 64 + lane];
-        }
-#pragma unroll 1
-        for (int k = 0; k < 8 && i0 + k * 64 < n; ++k) {
-          Entry c = e[0];
-#pragma unroll
-          for (int i = 1; i < 8; ++i)
-            if (i == k) c = e[i];
-          best.join(c.val, c.cls, top);
-        }
+        for (int k = 0; k < 8; ++k) gather(e[k].val >= least, e[k], found, count);
+        if ((i0 += 512) < n) read(i0);
       }
-      write_top(o, row, top, best, a.r, a.s);
+      __syncthreads();
+      if (count <= kWave) {
+        Entry e = {__builtin_nanf(""), 0};
+        if (lane < count) e = found[lane];
+        const int rank = rank_of(e, count);
+        if (rank < top) {
+          o.top_class[row * top + rank] = e.cls;
+          o.top_logp[row * top + rank] = logp_of(e.val, a.r, a.s == 0.f ? -kInf : logf(a.s));
+        }
+      } else {  // many equal ones
+        Top best;
+        for (int i = 0; i < n; i += 64) {
+          Entry e = {__builtin_nanf(""), 0};
+          if (i + lane < n) e = from[i + lane];
+          best.join(e.val, e.cls, top);
+        }
+        write_top(o, row, top, best, a.r, a.s);
+      }
+      __syncthreads();  // the next row's entries
     }
   }
 }

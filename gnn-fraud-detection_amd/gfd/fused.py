@@ -510,8 +510,9 @@ class ClassLogProbs(NamedTuple):
     top_classes: torch.Tensor            # [..., top]
 
 
-def _class_log_probs_fwd(logits, target, top, ignore_index):
-    """(logp, entropy, top_logp, top_class, statistics, the leading arguments of the C calls)."""
+def _class_log_probs_fwd(logits, target, top, ignore_index, keep=False):
+    """(logp, entropy, top_logp, top_class, statistics or None, the leading arguments of the C
+    calls)."""
     dev = logits.device
     rows, classes = logits.shape
     f32 = dict(dtype=torch.float32, device=dev)
@@ -519,13 +520,16 @@ def _class_log_probs_fwd(logits, target, top, ignore_index):
     entropy = torch.empty(rows, **f32)
     top_logp = torch.empty((rows, top), **f32)
     top_class = torch.empty((rows, top), dtype=torch.int64, device=dev)
-    stats = torch.empty((rows, 2), **f32)
     nbytes = _lib.load().gfd_class_logp_workspace_size(rows, classes, top)
-    ws = _ws(nbytes, dev) if nbytes else None
+    # statistics that nobody keeps lie behind the workspace: an allocation less
+    stats = torch.empty((rows, 2), **f32) if keep else None
+    behind = -(-nbytes // 16) * 16
+    ws = _ws(nbytes if keep else behind + 8 * rows, dev) if nbytes or not keep else None
     geom = (_ROW_DTYPES[logits.dtype], rows, classes, logits.stride(0))
     _lib.call_on(dev, "gfd_class_logp_fwd", logits.data_ptr(), *geom, _lib.ptr(target),
                  ignore_index, top, _lib.ptr(logp), entropy.data_ptr(), top_logp.data_ptr(),
-                 top_class.data_ptr(), stats.data_ptr(), _lib.ptr(ws), nbytes,
+                 top_class.data_ptr(), stats.data_ptr() if keep else ws.data_ptr() + behind,
+                 _lib.ptr(ws), nbytes,
                  _lib.stream_handle(dev))
     return logp, entropy, top_logp, top_class, stats, geom
 
@@ -537,7 +541,7 @@ class _ClassLogProbs(torch.autograd.Function):
     @staticmethod
     def forward(ctx, logits, target, top, ignore_index):
         logp, entropy, top_logp, top_class, stats, ctx.geom = _class_log_probs_fwd(
-            logits, target, top, ignore_index)
+            logits, target, top, ignore_index, True)
         ctx.save_for_backward(logits, target, entropy, top_class, stats)
         ctx.top, ctx.ignore_index = top, ignore_index
         ctx.mark_non_differentiable(top_class)

@@ -122,7 +122,7 @@ def test_rows(N, V):
 
 @pytest.mark.gpu
 @pytest.mark.parametrize("top", [0, 1, 2, 31, 32, 33, 63, 64])
-@pytest.mark.parametrize("V", [64, 100, 700, 9000])
+@pytest.mark.parametrize("V", [64, 100, 700, 9000, 300000])
 def test_top(top, V):
     check(logits(6, V, torch.bfloat16), targets(6, V), top)
 
