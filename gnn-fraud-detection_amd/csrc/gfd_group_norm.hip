@@ -151,6 +151,13 @@ __device__ __forceinline__ void affine(const void* p, int f32, int c, float none
 
 __device__ __forceinline__ float exp_of(float v) { return __builtin_amdgcn_exp2f(v * 1.4426950408889634f); }
 
+// a b - c, the product rounded like the one that c is a mean of: where c is that product alone, 0
+// and not what its rounding left
+__device__ __forceinline__ float less(float a, float b, float c) {
+#pragma clang fp contract(off)
+  return a * b - c;
+}
+
 // activation and, where d is not null, its derivative at z
 template <int ACT>
 __device__ __forceinline__ float activate(float z, float* d) {
@@ -241,7 +248,7 @@ struct Columns {
                                                  float rb) const {
     Pack<T, V> g;
 #pragma unroll
-    for (int j = 0; j < V; ++j) g.v[j] = from_f32<T>(fmaf(-xh[j], rb, fmaf(A[j], dz[j], -ra)));
+    for (int j = 0; j < V; ++j) g.v[j] = from_f32<T>(fmaf(-xh[j], rb, less(A[j], dz[j], ra)));
     return g;
   }
 };
@@ -587,7 +594,7 @@ __global__ void __launch_bounds__(kRowThreads) k_rows(const Norm n) {
         }
         const float ma = near_sum(sa, gv) * inv, mb = near_sum(sb, gv) * inv;
 #pragma unroll
-        for (int j = 0; j < V; ++j) o.v[j] = from_f32<T>(r * (fmaf(w[j], dz[j], -ma) - xh[j] * mb));
+        for (int j = 0; j < V; ++j) o.v[j] = from_f32<T>(r * (less(w[j], dz[j], ma) - xh[j] * mb));
       } else {
 #pragma unroll
         for (int j = 0; j < V; ++j) o.v[j] = from_f32<T>(activate<ACT>(z[j], nullptr));

@@ -299,6 +299,21 @@ def test_stream_and_graph():
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("act", ["none", "relu", "silu", "gelu"])
+def test_a_group_of_one_element_has_no_gradient(act):
+    """Its output is act(bias) wherever x is: w dz and its mean are one number."""
+    from gfd.fused import group_norm
+    w, b = affine(32, torch.float32)
+    for x, ptr in ((data((60, 32), torch.float32), None), (data((7, 1, 3), torch.float32), None),
+                   (data((60, 32), torch.float32), torch.arange(61, device=DEV))):
+        C = x.shape[-1]
+        xr, wr = x.requires_grad_(), w[:C].detach().requires_grad_()
+        y = group_norm(xr, C, wr, b[:C], act=act, ptr=ptr)
+        gx, gw = torch.autograd.grad(y, (xr, wr), data(x.shape, torch.float32, seed=5))
+        assert not gx.any() and not gw.any()
+
+
+@pytest.mark.gpu
 def test_offsets_past_32_bits():
     """The last rows of more than 2^31 elements give what they give alone: rows of their own, two
     long segments, and short ones behind a long one."""
