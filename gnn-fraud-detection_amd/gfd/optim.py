@@ -18,7 +18,8 @@ train.py:143): the same constructor arguments and update, over
   with the state dict of a ``torch.optim.Adam`` / ``AdamW``.
 * The step count is on the device, so ``step()`` can be captured into a graph
   (after one call outside of it, which makes the states) and every replay is a
-  step.  ``lr`` may be a 0-dim fp32 device tensor, which replays then follow.
+  step; ``mark_stepped()`` after replays lets what watches the parameters'
+  versions know.  ``lr`` may be a 0-dim fp32 device tensor, which replays then follow.
 """
 from __future__ import annotations
 
@@ -40,6 +41,7 @@ _grad, _dtype, _layout = attrgetter("grad"), attrgetter("dtype"), attrgetter("la
 _data_ptr, _numel, _device, _contiguous = (torch.Tensor.data_ptr, torch.Tensor.numel,
                                            torch.Tensor.get_device, torch.Tensor.is_contiguous)
 _NONE = type(None)
+_STATES = ("step", "exp_avg", "exp_avg_sq", "exp_avg_scale", "exp_avg_sq_scale")
 
 
 def _dense(p: torch.Tensor) -> bool:
@@ -232,6 +234,19 @@ class Adam(torch.optim.Optimizer):
                 self._step_group(group, self._group_state(gi))
         return loss
 
+    def mark_stepped(self) -> None:
+        """To be called after replays of a captured ``step()``: a replay writes the parameters
+        and states, but raises no version counter of theirs, by which autograd and what is
+        derived from parameters (the packed weights of an inference layer) notice a change."""
+        for gi, group in enumerate(self.param_groups):
+            self._raise_versions(self._flat.get(gi), group["params"])
+
+    @staticmethod
+    def _raise_versions(f, params: list) -> None:
+        # the flat buffers share theirs with the views of them
+        states = [f[k] for k in _STATES if k in f] if f is not None else []
+        torch.autograd.graph.increment_version(params + states)
+
     def _step_group(self, group: dict, f: dict) -> None:
         params = group["params"]
         grads = list(map(_grad, params))
@@ -249,6 +264,7 @@ class Adam(torch.optim.Optimizer):
             table[:, 0] = list(map(_data_ptr, params))
             table[:, 1] = list(map(_data_ptr, grads))
             self._launch(group, f, dtype, table)
+            self._raise_versions(f, params)
             return
         self._step_mixed(group, f)
 
@@ -259,6 +275,7 @@ class Adam(torch.optim.Optimizer):
         index = dev.index
         tables: Dict[torch.dtype, Tuple[list, list, list]] = {}
         kept = []                       # copies of gradients, alive until the launch is queued
+        stepped = []
         dtype = params = grads = places = None
         for i, p in enumerate(group["params"]):
             g = p.grad
@@ -280,11 +297,13 @@ class Adam(torch.optim.Optimizer):
             params.append(p.data_ptr())
             grads.append(g.data_ptr())
             places.append(i)
+            stepped.append(p)
         for dtype, (params, grads, places) in tables.items():
             table = f["table"][places]
             table[:, 0] = params
             table[:, 1] = grads
             self._launch(group, f, dtype, table)
+        self._raise_versions(f, stepped)
 
     def _launch(self, group: dict, f: dict, dtype: torch.dtype, table: np.ndarray) -> None:
         dev, lr, lr_ptr = f["device"], group["lr"], None

@@ -508,3 +508,92 @@ def test_c_argument_errors():
     for bad in ((0, 256, 8, 0, 0), (256, 0, 8, 0, 0), (256, 256, -1, 0, 0), (256, 256, 8, 100, 0),
                 (256, 256, 8, 0, -1), (257, 256, 8, 0, 0)):
         assert step(rows=(bad,)) == 1, bad
+
+
+class _Written:
+    """The library's calls in the place of a launch: what the step's Python does without a GPU."""
+
+    def __init__(self):
+        self.calls = []
+
+    def call(self, name, *args):
+        self.calls.append(name)
+
+    def call_on(self, device, name, *args):
+        self.calls.append(name)
+
+    def gfd_gat_packed_size(self, *shape):
+        return 64
+
+
+def _on_the_host(monkeypatch, params, **kw):
+    """An Adam over CPU parameters whose states are there and whose launches do nothing."""
+    import types
+
+    import numpy as np
+    from gfd import _lib, optim
+    calls = _Written()
+    for name in ("call", "call_on"):
+        monkeypatch.setattr(_lib, name, getattr(calls, name))
+    monkeypatch.setattr(_lib, "load", lambda: calls)
+    monkeypatch.setattr(_lib, "stream_handle", lambda device=None: 0)
+    opt = optim.Adam(params, **kw)
+    first = [0]
+    for p in params:
+        first.append(first[-1] + -(-p.numel() // BLOCK) * BLOCK)
+    f = {"first": first[:-1], "numel": [p.numel() for p in params], "bits": 32,
+         "device": types.SimpleNamespace(index=-1), "step": torch.zeros(len(params), dtype=torch.int32),
+         "ticket": torch.zeros(1056, dtype=torch.int32), "exp_avg": torch.zeros(first[-1]),
+         "exp_avg_sq": torch.zeros(first[-1]),
+         "table": np.array([(0, 0, p.numel(), at, i) for i, (p, at) in enumerate(zip(params, first))], dtype=np.int64)}
+    opt._flat[0] = f
+    for i, p in enumerate(params):
+        opt.state[p] = opt._views(f, i, p)
+    return opt, calls
+
+
+@pytest.mark.parametrize("missing", [False, True])
+def test_a_step_raises_the_versions_of_what_it_writes(monkeypatch, missing):
+    """What is derived from a parameter by its version (a layer's packed weights) is made again
+    after a step, and a backward pass through an overwritten parameter is refused, as after
+    torch's optimizers."""
+    from gfd import fused
+    from gfd import nn as gnn
+    conv = gnn.GATConv(16, 64, heads=8, concat=False)
+    params = list(conv.parameters())
+    opt, calls = _on_the_host(monkeypatch, params)
+    packed, _ = fused.eval_weights(conv, None, torch.device("cpu"))
+    for p in params:
+        p.grad = torch.ones_like(p)
+    if missing:
+        params[0].grad = None
+    versions = [p._version for p in params]
+    moments = opt.state[params[1]]["exp_avg"]._version
+    loss = (params[1] * params[1]).sum()
+    opt.step()
+    assert calls.calls.count("gfd_adam_step") == 1
+    assert [p._version - v for p, v in zip(params, versions)] == [0 if missing else 1] + [1] * (len(params) - 1)
+    assert opt.state[params[1]]["exp_avg"]._version > moments
+    assert fused.eval_weights(conv, None, torch.device("cpu"))[0] is not packed
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        loss.backward()
+
+
+def test_mark_stepped_raises_the_versions(monkeypatch):
+    """What a program calls after replays of a captured step, which raise none."""
+    p, q = torch.zeros(5, requires_grad=True), torch.zeros(7, requires_grad=True)
+    p.grad = torch.ones(5)
+    opt, calls = _on_the_host(monkeypatch, [p, q])
+    versions = p._version, opt.flat_state()["exp_avg"]._version
+    opt.mark_stepped()
+    assert p._version > versions[0] and opt.flat_state()["exp_avg"]._version > versions[1] and not calls.calls
+
+
+@pytest.mark.gpu
+def test_a_backward_pass_through_a_stepped_parameter_is_refused():
+    from gfd.optim import Adam
+    p, = make([300], torch.float32)
+    loss = (p * p).sum()
+    Adam([p]).step()
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        loss.backward()

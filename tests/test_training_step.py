@@ -252,3 +252,60 @@ def test_stream_of_any_form_of_a_device(monkeypatch):
     for device in ("cuda", "cuda:0", torch.device("cuda"), None):
         assert _lib.stream_handle(device) == 7 and seen.pop() == device
     assert _lib.stream_handle(torch.device("cuda", 2)) == 102 and not seen
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("norm", ["batch", "group"])
+@pytest.mark.parametrize("kind", ["GAT", "TemporalGNN"])
+def test_evaluation_follows_a_step(kind, norm):
+    """evaluate, step, evaluate: the second evaluation is a fresh model's of the same state."""
+    from gfd import models
+    from gfd.optim import AdamW
+    ei, x, y = (t.to(DEV) for t in _problem())
+
+    def make():
+        torch.manual_seed(3)
+        return getattr(models, kind)(WIDTH, 64, CLASSES, num_layers=2, dropout=0.0, norm=norm).to(DEV)
+
+    def evaluate(m):
+        with torch.no_grad():
+            return m.eval().log_probs(x, ei, y, top=2)
+
+    m = make()
+    opt = AdamW(m.parameters(), lr=1e-2)
+    before = evaluate(m)
+    for _ in range(2):
+        opt.zero_grad()
+        loss, _ = _loss(m.train(), ei, x, y)
+        loss.backward()
+        opt.step()
+        after, fresh = evaluate(m), make()
+        fresh.load_state_dict(m.state_dict())
+        for a, b in zip(after, evaluate(fresh)):
+            assert torch.equal(a, b)
+        assert not torch.equal(after.entropy, before.entropy)
+
+
+@pytest.mark.gpu
+def test_evaluation_follows_replays_of_a_captured_step():
+    from gfd.optim import AdamW
+    ei, x, y = (t.to(DEV) for t in _problem())
+    m, fresh = _model().to(DEV), _model().to(DEV)
+    opt = AdamW(m.parameters(), lr=1e-2)
+    for p in m.parameters():
+        p.grad = torch.full_like(p, 0.1)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        opt.step()
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        opt.step()
+    with torch.no_grad():
+        for _ in range(2):
+            m.eval()(x, ei)
+            graph.replay()
+            opt.mark_stepped()
+            fresh.load_state_dict(m.state_dict())
+            assert torch.equal(m.eval()(x, ei), fresh.eval()(x, ei))
