@@ -33,6 +33,7 @@ from __future__ import annotations
 from typing import NamedTuple, Optional, Tuple
 
 import torch
+from torch.autograd import forward_ad
 from torch.autograd.function import once_differentiable
 
 from . import _lib
@@ -447,7 +448,12 @@ class _GroupNorm(torch.autograd.Function):
 
 
 def _needs_grad(*tensors) -> bool:
-    return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)
+    """Whether autograd has to see a call: for a gradient, or, while a forward-mode level is open,
+    for a tangent, which the functions refuse."""
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
+        return True
+    return forward_ad._current_level >= 0 and any(
+        t is not None and forward_ad.unpack_dual(t).tangent is not None for t in tensors)
 
 
 def group_norm(x: torch.Tensor, num_groups: int, weight: Optional[torch.Tensor] = None,

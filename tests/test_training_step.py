@@ -309,3 +309,38 @@ def test_evaluation_follows_replays_of_a_captured_step():
             opt.mark_stepped()
             fresh.load_state_dict(m.state_dict())
             assert torch.equal(m.eval()(x, ei), fresh.eval()(x, ei))
+
+
+@pytest.mark.parametrize("place", range(3))
+def test_a_tangent_is_seen(place):
+    """Of any of the inputs, with and without gradients, and only while its level is open."""
+    from torch.autograd import forward_ad
+
+    from gfd.fused import _needs_grad
+    inputs = [torch.ones(4), None, torch.ones(4)]
+    with forward_ad.dual_level():
+        assert not _needs_grad(*inputs)
+        if inputs[place] is not None:
+            inputs[place] = forward_ad.make_dual(inputs[place], torch.ones(4))
+        assert _needs_grad(*inputs) == (inputs[place] is not None)
+        with torch.no_grad():
+            assert _needs_grad(*inputs) == (inputs[place] is not None)
+    assert not _needs_grad(*inputs) and not _needs_grad(None)
+
+
+@pytest.mark.gpu
+def test_forward_mode_is_refused():
+    """Neither operator has a forward-mode derivative: an input with a tangent is an error, not a
+    result without one."""
+    from torch.autograd import forward_ad
+
+    from gfd.fused import class_log_probs, group_norm
+    x, w = torch.randn(5, 8, device=DEV), torch.ones(8, device=DEV)
+    with forward_ad.dual_level():
+        d, dw = (forward_ad.make_dual(t, torch.ones_like(t)) for t in (x, w))
+        for call in (lambda: group_norm(d, 2), lambda: group_norm(d[None], 2, w), lambda: group_norm(x, 2, dw),
+                     lambda: group_norm(x, 2, w, dw), lambda: class_log_probs(d, top=1),
+                     lambda: class_log_probs(d[0])):
+            with pytest.raises(NotImplementedError):
+                call()
+        assert forward_ad.unpack_dual(group_norm(x, 2)).tangent is None
