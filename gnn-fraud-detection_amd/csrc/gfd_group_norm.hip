@@ -551,7 +551,9 @@ __global__ void __launch_bounds__(kRowThreads) k_rows(const Norm n) {
       }
       const float off = near_sum(s1, gv) * inv;
       const float var = fmaxf(fmaf(-off, off, near_sum(s2, gv) * inv), 0.f);
-      const float r = rsqrtf(var + float(n.eps)), lr = off * r;
+      // a row beyond the last, whose variance of 0 an eps of 0 leaves, adds 0 to the column sums
+      const float r = BWD && r0 + u * step >= n.segments ? 0.f : rsqrtf(var + float(n.eps));
+      const float lr = off * r;
       float xh[V], z[V];
       bool near = false;
 #pragma unroll

@@ -601,7 +601,8 @@ gfd_status gfd_rows_copy(const float* src, int64_t src_stride, const int32_t* sr
  * grad_x) contiguous in the rows' order.  weight / bias [channels], nullable
  * (identity), w_dtype F32 or x's.  Sums are fp64, or fp32 over a few rows about
  * one of their elements, which fp64 joins: a level far above the spread costs no
- * digits, and deviations whose squares leave fp32 (about 1e19) are not served.
+ * digits, and deviations whose squares leave fp32 (about 1e19, and with eps 0 below
+ * 1e-19) are not served.
  * stats (fp64 [segments, groups, 2] = mean, 1/sqrt(var + eps)) is nullable in the forward
  * and what the backward takes; dense segments of one row keep none (stats NULL:
  * the backward finds them again).  channels <= 2048 and a multiple of groups.

@@ -416,3 +416,15 @@ def test_c_argument_errors():
     assert fwd(channels=4096, groups=1) == 5 and fwd(segments=-1) == 1 and fwd(stride=-8) == 1
     assert fwd(length=0) == 0 and fwd(segments=0) == 0         # nothing to do
     assert fwd(length=100000) == 3                             # no workspace
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("act", ["none", "relu", "silu", "gelu"])
+@pytest.mark.parametrize("shape", [(1, 64), (5, 64), (300, 32), (4100, 24), (17, 1, 24), (70, 15), (9, 40, 24),
+                                   (2, 3000, 16)])
+def test_an_eps_of_zero(shape, act):
+    """Outputs and all gradients, at row counts that leave the last blocks' rows in part unused."""
+    C = shape[-1]
+    for dtype in (torch.float32, torch.bfloat16):
+        check(data(shape, dtype), C // 8 if C % 8 == 0 else 3, *affine(C, torch.float32), act=act, eps=0.0)
+        check(data(shape, dtype), C // 8 if C % 8 == 0 else 3, *affine(C, torch.float32), act=act, eps=1e-60)
