@@ -171,32 +171,55 @@ class Adam(torch.optim.Optimizer):
     @torch.no_grad()
     def load_state_dict(self, state_dict: dict) -> None:
         """Of this class, or of torch.optim.Adam / AdamW (fp32 states).  One that is refused leaves
-        the optimizer as it was."""
+        the optimizer as it was.  States of the same ``state_bits`` are filled where they are, and
+        so is an lr that is a tensor: a captured ``step()`` goes on from what was loaded (but for the numbers
+        among the options, which it holds).  With other ``state_bits`` the states are made anew,
+        and a captured step has to be captured again."""
         groups = []
         for g, mine in zip(state_dict["param_groups"], self.param_groups):
             groups.append({**{k: mine[k] for k in ("state_bits", "seed", "decoupled_weight_decay")}, **g})
         if len(groups) != len(state_dict["param_groups"]):
             raise ValueError("loaded state dict has a different number of parameter groups")
         before = self._flat, self.state, self.param_groups
+        copies = []                     # (to, from) of everything that is kept, once nothing is refused
         try:
             super().load_state_dict({"state": {}, "param_groups": groups})
             self._flat, self.state = {}, defaultdict(dict)
-            self._fill_groups(groups, state_dict)
+            for gi, saved in enumerate(groups):
+                self._load_group(gi, saved["params"], state_dict["state"], before, copies)
         except Exception:
             self._flat, self.state, self.param_groups = before
             raise
+        for to, t in copies:
+            to.copy_(t) if t is not None else to.zero_()
 
-    def _fill_groups(self, groups: list, state_dict: dict) -> None:
-        for gi, (group, saved) in enumerate(zip(self.param_groups, groups)):
-            self._check_group(group)
-            if not any(k in state_dict["state"] for k in saved["params"]):
-                continue
+    def _load_group(self, gi: int, keys: list, states: dict, before: tuple, copies: list) -> None:
+        flat, state, old_groups = before
+        group, old, f = self.param_groups[gi], old_groups[gi], flat.get(gi)
+        self._check_group(group)
+        known = any(k in states for k in keys)
+        # one that cannot be gone on with (other bits, parameters added, moved or laid out anew) is
+        # made anew
+        if (f is not None and f["bits"] == group["state_bits"] and len(f["first"]) == len(group["params"]) and
+                all(p.get_device() == f["device"].index and state[p]["exp_avg"].shape == p.shape and
+                    state[p]["exp_avg"].stride() == p.stride() for p in group["params"])):
+            self._flat[gi] = f
+            for p in group["params"]:
+                self.state[p] = state[p]
+        elif known:
             self._group_state(gi)
-            for p, k in zip(group["params"], saved["params"]):
-                if k in state_dict["state"]:
-                    self._fill(group, p, state_dict["state"][k])
+        if gi in self._flat:
+            for p, k in zip(group["params"], keys):
+                copies += (self._loaded(group, p, states[k]) if k in states else
+                           [(to, None) for to in self.state[p].values()])
+        lr = old["lr"]
+        if isinstance(lr, torch.Tensor):
+            copies.append((lr, torch.as_tensor(group["lr"])))
+            group["lr"] = lr
 
-    def _fill(self, group: dict, p: torch.Tensor, old: dict) -> None:
+    def _loaded(self, group: dict, p: torch.Tensor, old: dict) -> list:
+        """(to, from) of a parameter's states; says which one does not fit."""
+        copies = []
         for name, to in self.state[p].items():
             if name not in old:
                 raise ValueError(f"gfd Adam: the loaded state has no {name!r} (its states are not "
@@ -205,7 +228,8 @@ class Adam(torch.optim.Optimizer):
             if t.shape != to.shape or (t.dtype.itemsize == 1 or to.dtype.itemsize == 1) and t.dtype != to.dtype:
                 raise ValueError(f"gfd Adam: the loaded {name!r} is {t.dtype} {tuple(t.shape)}, "
                                  f"expected {to.dtype} {tuple(to.shape)}")
-            to.copy_(t)
+            copies.append((to, t))
+        return copies
 
     @torch.no_grad()
     def __setstate__(self, state: dict) -> None:
@@ -218,7 +242,8 @@ class Adam(torch.optim.Optimizer):
             if old:
                 self._group_state(gi)
                 for p, s in old.items():
-                    self._fill(group, p, s)
+                    for to, t in self._loaded(group, p, s):
+                        to.copy_(t)
 
     # -- the step -----------------------------------------------------------
 

@@ -597,3 +597,92 @@ def test_a_backward_pass_through_a_stepped_parameter_is_refused():
     Adam([p]).step()
     with pytest.raises(RuntimeError, match="modified by an inplace operation"):
         loss.backward()
+
+
+def test_a_load_fills_the_states_where_they_are(monkeypatch):
+    """A captured step holds their addresses, and that of a tensor lr; one that is refused
+    changes neither."""
+    params = [torch.zeros(300, requires_grad=True), torch.zeros((7, 5), requires_grad=True)]
+    lr = torch.tensor(0.5)
+    opt, _ = _on_the_host(monkeypatch, params, lr=lr)
+    for k, t in opt.flat_state().items():
+        t.copy_(torch.arange(t.numel()))
+    saved = copy.deepcopy(opt.state_dict())
+    saved["param_groups"][0]["lr"].fill_(0.25)
+    del saved["state"][1]
+    where = {k: t.data_ptr() for k, t in opt.flat_state().items()}
+    for t in opt.flat_state().values():
+        t.fill_(9)
+    bad = copy.deepcopy(saved)
+    bad["state"][0]["exp_avg_sq"] = torch.zeros(3)
+    with pytest.raises(ValueError, match="exp_avg_sq"):
+        opt.load_state_dict(bad)
+    assert lr == 0.5 and all((t == 9).all() for t in opt.flat_state().values())
+    for _ in range(2):
+        opt.load_state_dict(saved)
+        assert {k: t.data_ptr() for k, t in opt.flat_state().items()} == where
+        assert opt.param_groups[0]["lr"] is lr and lr == 0.25
+        for name in ("exp_avg", "exp_avg_sq"):
+            s = [opt.state[p][name] for p in params]
+            assert torch.equal(s[0], torch.arange(300.0)) and not s[1].any() and s[1].shape == (7, 5)
+        assert opt.flat_state()["step"].tolist() == [0, 0]
+        opt.state[params[1]]["exp_avg"].fill_(3.0)
+    saved["param_groups"][0]["lr"] = 0.125          # a number goes into the tensor
+    opt.load_state_dict(saved)
+    assert opt.param_groups[0]["lr"] is lr and lr == 0.125
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("bits", [32, 8])
+def test_replays_go_on_from_a_loaded_state(bits):
+    from gfd.optim import AdamW
+
+    def fresh():
+        params = make([5000, (33, 7)], torch.float32)
+        return params, AdamW(params, lr=torch.tensor(0.1, device=DEV), state_bits=bits, seed=3)
+
+    (a, captured), (b, eager) = fresh(), fresh()
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        captured.step()
+    torch.cuda.current_stream().wait_stream(side)
+    eager.step()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        captured.step()
+    saved = copy.deepcopy(eager.state_dict())
+    saved["param_groups"][0]["lr"].fill_(0.02)
+    saved["state"][0]["step"] += 5
+    for _ in range(3):
+        captured.load_state_dict(saved)
+        eager.load_state_dict(saved)
+        torch.full((20000,), float("nan"), device=DEV)     # memory that a load would have given back
+        for _ in range(2):
+            graph.replay()
+            eager.step()
+        torch.cuda.synchronize()
+        for p, q in zip(a, b):
+            assert torch.equal(p, q)
+            for k, t in captured.state[p].items():
+                assert torch.equal(t.float(), eager.state[q][k].float()), k
+    assert eager.state[b[0]]["step"].item() == 8 and torch.equal(eager.param_groups[0]["lr"],
+                                                                 captured.param_groups[0]["lr"])
+
+
+@pytest.mark.gpu
+def test_a_load_with_other_bits_makes_the_states_anew():
+    from gfd.optim import Adam
+    p, = make([700], torch.float32)
+    opt = Adam([p], lr=0.1)
+    opt.step()
+    q, = make([700], torch.float32)
+    other = Adam([q], lr=0.1, state_bits=8)
+    other.step()
+    opt.load_state_dict(other.state_dict())
+    assert opt.state[p]["exp_avg"].dtype == torch.float8_e4m3fn
+    with torch.no_grad():
+        p.copy_(q)
+    opt.step()
+    other.step()
+    assert torch.equal(p, q)
