@@ -394,24 +394,30 @@ def _check_rows(what: str, name: str, t: torch.Tensor) -> None:
         raise TypeError(f"gfd {what}: {name} must be float32, bfloat16 or float16 (got {t.dtype})")
 
 
+def _norm_geometry(x, weight, bias, ptr, groups) -> tuple:
+    """The shape arguments of the group norm's C calls: (before the affine tensors, GFD_DTYPE_* of
+    these)."""
+    segments, length = (ptr.numel() - 1, x.size(0)) if ptr is not None else (x.size(0), x.size(1))
+    w_dtype = weight.dtype if weight is not None else bias.dtype if bias is not None else x.dtype
+    return ((_ROW_DTYPES[x.dtype], segments, length, _lib.ptr(ptr), x.size(-1), groups, x.stride(-2),
+             0 if ptr is not None else x.stride(0)), _ROW_DTYPES[w_dtype])
+
+
 def _group_norm_fwd(x, weight, bias, ptr, groups, eps, act, keep):
-    """(y, statistics or None, the leading arguments of the C calls, GFD_DTYPE_* of the affine)."""
+    """(y, statistics or None)."""
     dev, ragged, C = x.device, ptr is not None, x.size(-1)
-    segments, length = (ptr.numel() - 1, x.size(0)) if ragged else (x.size(0), x.size(1))
+    geom, w_dtype = _norm_geometry(x, weight, bias, ptr, groups)
+    segments, length = geom[1:3]
     y = torch.empty(x.shape, dtype=x.dtype, device=dev)
     # a row of its own keeps no statistics: the backward finds them again
     stats = (torch.empty((segments, groups, 2), dtype=torch.float64, device=dev)
              if keep and (ragged or length != 1) else None)
-    geom = (_ROW_DTYPES[x.dtype], segments, length, _lib.ptr(ptr), C, groups, x.stride(-2),
-            0 if ragged else x.stride(0))
-    w_dtype = _ROW_DTYPES[weight.dtype if weight is not None else
-                          bias.dtype if bias is not None else x.dtype]
     nbytes = _lib.load().gfd_group_norm_workspace_size(segments, length, int(ragged), C, groups, 0)
     ws = _ws(nbytes, dev) if nbytes else None
     _lib.call_on(dev, "gfd_group_norm_fwd", x.data_ptr(), *geom, _lib.ptr(weight), _lib.ptr(bias),
                  w_dtype, eps, act, y.data_ptr(), _lib.ptr(stats), _lib.ptr(ws), nbytes,
                  _lib.stream_handle(dev))
-    return y, stats, geom, w_dtype
+    return y, stats
 
 
 class _GroupNorm(torch.autograd.Function):
@@ -421,30 +427,42 @@ class _GroupNorm(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx, x, weight, bias, ptr, groups, eps, act):
-        y, stats, ctx.geom, ctx.w_dtype = _group_norm_fwd(x, weight, bias, ptr, groups, eps, act, True)
+        y, stats = _group_norm_fwd(x, weight, bias, ptr, groups, eps, act, True)
         ctx.save_for_backward(x, weight, bias, ptr, stats)
-        ctx.act, ctx.eps = act, eps
+        ctx.groups, ctx.act, ctx.eps = groups, act, eps
         return y
 
     @staticmethod
     @once_differentiable
     def backward(ctx, grad):
+        # saved-tensor hooks may bring them back elsewhere and in other strides
         x, weight, bias, ptr, stats = ctx.saved_tensors
+        x = _unit_rows(x)
+        weight, bias, ptr, stats = map(_packed, (weight, bias, ptr, stats))
         dev = x.device
         grad = grad.contiguous()
         gx = torch.empty(x.shape, dtype=x.dtype, device=dev)
         gw = torch.empty_like(weight) if weight is not None and ctx.needs_input_grad[1] else None
         gb = torch.empty_like(bias) if bias is not None and ctx.needs_input_grad[2] else None
-        lib = _lib.load()
-        _, segments, length, _, C, groups, _, _ = ctx.geom
-        nbytes = lib.gfd_group_norm_workspace_size(segments, length, int(ptr is not None), C,
-                                                   groups, 1)
+        geom, w_dtype = _norm_geometry(x, weight, bias, ptr, ctx.groups)
+        nbytes = _lib.load().gfd_group_norm_workspace_size(*geom[1:3], int(ptr is not None), x.size(-1),
+                                                           ctx.groups, 1)
         ws = _ws(nbytes, dev)
-        _lib.call_on(dev, "gfd_group_norm_bwd", x.data_ptr(), *ctx.geom, _lib.ptr(weight),
-                     _lib.ptr(bias), ctx.w_dtype, ctx.eps, ctx.act, _lib.ptr(stats), grad.data_ptr(),
+        _lib.call_on(dev, "gfd_group_norm_bwd", x.data_ptr(), *geom, _lib.ptr(weight),
+                     _lib.ptr(bias), w_dtype, ctx.eps, ctx.act, _lib.ptr(stats), grad.data_ptr(),
                      gx.data_ptr(), _lib.ptr(gw), _lib.ptr(gb), ws.data_ptr(), ws.numel(),
                      _lib.stream_handle(dev))
         return gx, gw, gb, None, None, None, None
+
+
+def _packed(t):
+    """``t`` contiguous (None for None)."""
+    return t if t is None else t.contiguous()
+
+
+def _unit_rows(t: torch.Tensor) -> torch.Tensor:
+    """``t`` whose last dimension has no gaps."""
+    return t if t.size(-1) <= 1 or t.stride(-1) == 1 else t.contiguous()
 
 
 def _needs_grad(*tensors) -> bool:
@@ -499,10 +517,7 @@ def group_norm(x: torch.Tensor, num_groups: int, weight: Optional[torch.Tensor] 
     shape = x.shape
     if ptr is None:
         x = x.unsqueeze(1) if x.dim() == 2 else x.flatten(1, -2)
-    if C > 1 and x.stride(-1) != 1:
-        x = x.contiguous()
-    weight = weight.contiguous() if weight is not None else None
-    bias = bias.contiguous() if bias is not None else None
+    x, weight, bias = _unit_rows(x), _packed(weight), _packed(bias)
     args = (x, weight, bias, ptr, int(num_groups), float(eps), ACTIVATIONS[act])
     y = _GroupNorm.apply(*args) if _needs_grad(x, weight, bias) else _group_norm_fwd(*args, False)[0]
     return y if y.shape == shape else y.view(shape)
@@ -517,8 +532,7 @@ class ClassLogProbs(NamedTuple):
 
 
 def _class_log_probs_fwd(logits, target, top, ignore_index, keep=False):
-    """(logp, entropy, top_logp, top_class, statistics or None, the leading arguments of the C
-    calls)."""
+    """(logp, entropy, top_logp, top_class, statistics or None)."""
     dev = logits.device
     rows, classes = logits.shape
     f32 = dict(dtype=torch.float32, device=dev)
@@ -531,13 +545,12 @@ def _class_log_probs_fwd(logits, target, top, ignore_index, keep=False):
     stats = torch.empty((rows, 2), **f32) if keep else None
     behind = -(-nbytes // 16) * 16
     ws = _ws(nbytes if keep else behind + 8 * rows, dev) if nbytes or not keep else None
-    geom = (_ROW_DTYPES[logits.dtype], rows, classes, logits.stride(0))
-    _lib.call_on(dev, "gfd_class_logp_fwd", logits.data_ptr(), *geom, _lib.ptr(target),
-                 ignore_index, top, _lib.ptr(logp), entropy.data_ptr(), top_logp.data_ptr(),
-                 top_class.data_ptr(), stats.data_ptr() if keep else ws.data_ptr() + behind,
-                 _lib.ptr(ws), nbytes,
+    _lib.call_on(dev, "gfd_class_logp_fwd", logits.data_ptr(), _ROW_DTYPES[logits.dtype], rows,
+                 classes, logits.stride(0), _lib.ptr(target), ignore_index, top, _lib.ptr(logp),
+                 entropy.data_ptr(), top_logp.data_ptr(), top_class.data_ptr(),
+                 stats.data_ptr() if keep else ws.data_ptr() + behind, _lib.ptr(ws), nbytes,
                  _lib.stream_handle(dev))
-    return logp, entropy, top_logp, top_class, stats, geom
+    return logp, entropy, top_logp, top_class, stats
 
 
 class _ClassLogProbs(torch.autograd.Function):
@@ -546,7 +559,7 @@ class _ClassLogProbs(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx, logits, target, top, ignore_index):
-        logp, entropy, top_logp, top_class, stats, ctx.geom = _class_log_probs_fwd(
+        logp, entropy, top_logp, top_class, stats = _class_log_probs_fwd(
             logits, target, top, ignore_index, True)
         ctx.save_for_backward(logits, target, entropy, top_class, stats)
         ctx.top, ctx.ignore_index = top, ignore_index
@@ -557,15 +570,17 @@ class _ClassLogProbs(torch.autograd.Function):
     @staticmethod
     @once_differentiable
     def backward(ctx, g_logp, g_entropy, g_top, _):
+        # saved-tensor hooks may bring them back elsewhere and in other strides
         logits, target, entropy, top_class, stats = ctx.saved_tensors
+        logits = _unit_rows(logits)
+        target, entropy, top_class, stats = map(_packed, (target, entropy, top_class, stats))
         dev = logits.device
-        g_logp, g_entropy, g_top = (g.contiguous() if g is not None else None
-                                    for g in (g_logp, g_entropy, g_top))
+        g_logp, g_entropy, g_top = map(_packed, (g_logp, g_entropy, g_top))
         grad = torch.empty(logits.shape, dtype=logits.dtype, device=dev)
-        _lib.call_on(dev, "gfd_class_logp_bwd", logits.data_ptr(), *ctx.geom, _lib.ptr(target),
-                     ctx.ignore_index, ctx.top, top_class.data_ptr(), stats.data_ptr(),
-                     entropy.data_ptr(), _lib.ptr(g_logp), _lib.ptr(g_entropy), _lib.ptr(g_top),
-                     grad.data_ptr(), _lib.stream_handle(dev))
+        _lib.call_on(dev, "gfd_class_logp_bwd", logits.data_ptr(), _ROW_DTYPES[logits.dtype],
+                     *logits.shape, logits.stride(0), _lib.ptr(target), ctx.ignore_index, ctx.top,
+                     top_class.data_ptr(), stats.data_ptr(), entropy.data_ptr(), _lib.ptr(g_logp),
+                     _lib.ptr(g_entropy), _lib.ptr(g_top), grad.data_ptr(), _lib.stream_handle(dev))
         return grad, None, None, None
 
 
@@ -598,8 +613,7 @@ def class_log_probs(logits: torch.Tensor, target: Optional[torch.Tensor] = None,
                              f"{tuple(target.shape)})")
         target = target.reshape(-1).contiguous()
     x = logits if logits.dim() == 2 else logits.reshape(-1, classes)
-    if (classes > 1 and x.stride(1) != 1) or x.stride(0) < 0:
-        x = x.contiguous()
+    x = _unit_rows(x)
     args = (x, target, int(top), int(ignore_index))
     logp, entropy, top_logp, top_class = (_ClassLogProbs.apply(*args) if _needs_grad(x) else
                                           _class_log_probs_fwd(*args)[:4])

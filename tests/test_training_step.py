@@ -344,3 +344,91 @@ def test_forward_mode_is_refused():
             with pytest.raises(NotImplementedError):
                 call()
         assert forward_ad.unpack_dual(group_norm(x, 2)).tangent is None
+
+
+class _Calls:
+    """The library's calls in the place of their launches."""
+
+    def __init__(self):
+        self.args = {}
+
+    def call_on(self, device, name, *args):
+        self.args[name] = args
+
+    def gfd_group_norm_workspace_size(self, *shape):
+        return 16
+
+    def gfd_class_logp_workspace_size(self, *shape):
+        return 0
+
+
+def _elsewhere(t):
+    """A copy with other strides: of rows at a larger pitch."""
+    if t.dim() != 2:
+        return torch.stack((t, t), -1)[..., 0] if t.dim() == 1 else t.clone()
+    return torch.cat((t, t[:, :1]), 1)[:, :-1]
+
+
+def test_saved_tensors_that_come_back_elsewhere(monkeypatch):
+    """Saved-tensor hooks (offloading, checkpoints) hand the backward copies: their addresses and
+    strides go to the library, not those of the forward's tensors."""
+    from gfd import _lib, fused
+    calls = _Calls()
+    monkeypatch.setattr(_lib, "call_on", calls.call_on)
+    monkeypatch.setattr(_lib, "load", lambda: calls)
+    monkeypatch.setattr(_lib, "stream_handle", lambda device=None: 0)
+    came = []
+
+    def unpack(t):
+        came.append(_elsewhere(t))
+        return came[-1]
+
+    x = torch.randn(40, 12)[:, 2:10].requires_grad_()
+    w, ptr = torch.ones(8, requires_grad=True), torch.tensor([0, 3, 40])
+    with torch.autograd.graph.saved_tensors_hooks(lambda t: t, unpack):
+        y = fused._GroupNorm.apply(x, w, None, ptr, 2, 1e-5, 1)
+        y.backward(torch.ones(40, 8))
+    a = calls.args["gfd_group_norm_bwd"]
+    assert calls.args["gfd_group_norm_fwd"][4] == ptr.data_ptr() != a[4]
+    assert a[0] in [t.data_ptr() for t in came if t.stride() == (9, 1)] and a[7:9] == (9, 0)
+    assert a[1:4] == (0, 2, 40) and a[5:7] == (8, 2) and a[9] != w.data_ptr()
+    came.clear()
+    x.grad = None
+    with torch.autograd.graph.saved_tensors_hooks(lambda t: t, unpack):
+        logp, entropy, _, _ = fused._ClassLogProbs.apply(x, torch.zeros(40, dtype=torch.int64), 2, -1)
+        (logp.sum() + entropy.sum()).backward()
+    f, a = calls.args["gfd_class_logp_fwd"], calls.args["gfd_class_logp_bwd"]
+    assert f[:5] == (x.data_ptr(), 0, 40, 8, 12) and a[1:5] == (0, 40, 8, 9)
+    assert a[0] in [t.data_ptr() for t in came if t.stride() == (9, 1)] and a[5] != f[5]
+
+
+@pytest.mark.gpu
+def test_offloaded_and_checkpointed_passes_give_the_same_gradients():
+    from torch.utils.checkpoint import checkpoint
+
+    from gfd.fused import class_log_probs, group_norm
+    base = torch.randn(300, 70, device=DEV)
+    ptr = torch.tensor([0, 0, 5, 5, 200, 0, 290, 0], device=DEV)[::2]     # a copy of it is taken
+    t = torch.randint(-1, 64, (300,), device=DEV)
+    w = torch.rand(64, device=DEV)
+
+    def passes(x, w):
+        h = group_norm(x, 8, w, act="silu", ptr=ptr)
+        r = class_log_probs(group_norm(h, 8) * 2, t, top=3)
+        s = class_log_probs(x, t, top=1)
+        return r.log_prob.sum() + r.entropy.sum() + s.log_prob.sum() + 0.5 * s.top_log_probs.sum()
+
+    def grads(run):
+        leaf, lw = base.clone().requires_grad_(), w.clone().requires_grad_()
+        return torch.autograd.grad(run(leaf[:, 3:67], lw), (leaf, lw))
+
+    def offloaded(x, w):
+        with torch.autograd.graph.save_on_cpu():
+            return passes(x, w)
+
+    want = grads(passes)
+    for run in (offloaded, lambda x, w: checkpoint(passes, x, w, use_reentrant=False)):
+        for a, b in zip(grads(run), want):
+            # another alignment is another order of a row's fp32 sums: 48 roundings, for each of
+            # the three passes
+            assert_close_scaled(a, b, rtol=3 * 48 * 2.0 ** -24)
