@@ -48,7 +48,7 @@ struct Norm {
   const void* w;
   const void* b;
   double* stats;   // [segments, groups, 2]
-  double2* part;   // forward: column sums of x and x^2
+  double2* part;   // forward: column sums of x - c and (x - c)^2, c: base_of
   float2* grad_part;  // backward: of dz and dz xhat
   double2* mom;    // backward: A, B of a segment and group
   void* dw;        // backward, nullable
@@ -99,6 +99,7 @@ __device__ __forceinline__ int64_t segment_of(const Norm& n, int64_t r) {
 
 struct Piece {
   int64_t seg, r0, r1;  // rows [r0, r1) of segment seg, none where r0 >= r1
+  int64_t start;        // of the segment
 };
 
 // piece i (ragged: 0 or 1) of the long segments in tile t; its sums go to row 2 t + i (ragged) or
@@ -107,11 +108,12 @@ __device__ __forceinline__ Piece piece_of(const Norm& n, int64_t t, int i) {
   const int64_t a = t * n.tile, e = a + n.tile < n.length ? a + n.tile : n.length;
   if (!n.ptr) {
     const int64_t s = blockIdx.z, base = s * n.length;
-    return {s, base + a, base + e};
+    return {s, base + a, base + e, base};
   }
-  Piece p = {segment_of(n, i == 0 ? a : e - 1), 0, 0};
+  Piece p = {segment_of(n, i == 0 ? a : e - 1), 0, 0, 0};
   if (p.seg < 0) return p;
   segment_rows(n, p.seg, p.r0, p.r1);
+  p.start = p.r0;
   // the second is the one that starts inside the tile
   if (p.r1 - p.r0 <= n.tile || (i == 1 && p.r0 <= a)) p.r1 = p.r0;
   p.r0 = p.r0 < a ? a : p.r0;
@@ -124,6 +126,14 @@ __device__ __forceinline__ const T* row_in(const Norm& n, const void* base, int6
   const T* p = static_cast<const T*>(base);
   return n.ptr ? p + r * n.row_stride
                : p + seg * n.seg_stride + (r - seg * n.length) * n.row_stride;
+}
+
+// what the sums of a segment (with rows, the first one ``start``) and a group are taken about in
+// fp64: its first element.  However far from 0 the group lies, the sum of squares is at most its
+// number of elements times the spread's, so that of 53 bits only as many go as that number has
+template <typename T>
+__device__ __forceinline__ double base_of(const Norm& n, int64_t seg, int64_t start, int group) {
+  return double(to_f32(row_in<T>(n, n.x, seg, start)[group * (n.channels / n.groups)]));
 }
 
 // ---------------------------------------------------------------------------
@@ -253,12 +263,12 @@ struct Columns {
   }
 };
 
-// mean and 1 / sqrt(var + eps) from the sums of x and x^2 over n elements
-__device__ __forceinline__ double2 moments_of(double s, double q, double n, double eps) {
+// mean and 1 / sqrt(var + eps) from the sums of x - c and (x - c)^2 over n elements
+__device__ __forceinline__ double2 moments_of(double s, double q, double n, double eps, double c) {
   const double mean = s / n;
   double var = q / n - mean * mean;
   if (var < 0.0) var = 0.0;
-  return {mean, 1.0 / sqrt(var + eps)};
+  return {c + mean, 1.0 / sqrt(var + eps)};
 }
 
 // the sum over the threads of a block that share a column (threadIdx.x % cols), in those of the
@@ -283,7 +293,7 @@ __device__ __forceinline__ double2 sum_rows(double2 v, int cols, double2* red) {
   return v;
 }
 
-// A thread's sums of x and x^2, in fp32 about its own first element k and, every few rows, into
+// A thread's sums of x and x^2 about c, in fp32 about its own first element k and, every few rows, into
 // fp64 (a conversion to fp64 takes four times an fp32 operation): what rounding does to the
 // deviations from k, however far k lies from 0, is not multiplied by it.  The squares of the k -
 // mean of all threads are at most the sum of squares itself, so neither does an odd k cost digits.
@@ -302,10 +312,10 @@ struct Shifted {
     s = q = 0.f;
     n += count;
   }
-  // the sums themselves
-  __device__ __forceinline__ double2 sums() const {
-    const double c = double(k), m = double(n);
-    return {fma(m, c, a), fma(c, fma(m, c, 2.0 * a), b)};
+  // about c
+  __device__ __forceinline__ double2 sums(double c) const {
+    const double d = double(k) - c, m = double(n);
+    return {fma(m, d, a), fma(d, fma(m, d, 2.0 * a), b)};
   }
 };
 
@@ -344,7 +354,8 @@ __device__ __forceinline__ void do_team(const Norm& n, uint32_t block, uint32_t 
       return v;
     };
     // sums over the rows by column (f(k, col, a, b) adds a thread's), then of each group, handed
-    // to done(segment, group, a, b, its number of elements) and left at its first column
+    // to done(segment, its first row, group, a, b, its number of elements) and left at its first
+    // column
     auto reduce = [&](auto f, auto done) {
 #pragma unroll
       for (int k = 0; k < NC; ++k) {
@@ -374,7 +385,7 @@ __device__ __forceinline__ void do_team(const Norm& n, uint32_t block, uint32_t 
           a += cs[k].x;
           b += cs[k].y;
         }
-        cs[0] = done(s0 + tm, g, a, b, double(q1 - q0) * (n.channels / n.groups));
+        cs[0] = done(s0 + tm, q0, g, a, b, double(q1 - q0) * (n.channels / n.groups));
       }
       __syncthreads();
     };
@@ -392,12 +403,12 @@ __device__ __forceinline__ void do_team(const Norm& n, uint32_t block, uint32_t 
               for (int j = 0; j < V; ++j) t.add(x.at(j));
               t.fold(V);
             }
-            const double2 v = t.sums();
+            const double2 v = t.sums(base_of<T>(n, seg, r0, col / gv));
             a = v.x;
             b = v.y;
           },
-          [&](int64_t s, int g, double a, double b, double count) {
-            const double2 m = moments_of(a, b, count, n.eps);
+          [&](int64_t s, int64_t start, int g, double a, double b, double count) {
+            const double2 m = moments_of(a, b, count, n.eps, base_of<T>(n, s, start, g));
             if (!BWD && n.stats) {
               n.stats[2 * (s * n.groups + g)] = m.x;
               n.stats[2 * (s * n.groups + g) + 1] = m.y;
@@ -436,7 +447,7 @@ __device__ __forceinline__ void do_team(const Norm& n, uint32_t block, uint32_t 
               b += double(sb);
             }
           },
-          [&](int64_t, int, double a, double b, double count) { return double2{a / count, b / count}; });
+          [&](int64_t, int64_t, int, double a, double b, double count) { return double2{a / count, b / count}; });
 #pragma unroll
       for (int k = 0; k < NC; ++k) {
         const int col = c + k * n.cols;
@@ -566,14 +577,15 @@ __global__ void __launch_bounds__(kRowThreads) k_rows(const Norm n) {
         double ds = 0.0, dq = 0.0;
 #pragma unroll
         for (int j = 0; j < V; ++j) {
-          ds += double(x[u].at(j));
-          dq += double(x[u].at(j)) * double(x[u].at(j));
+          const double t = double(x[u].at(j)) - double(m);
+          ds += t;
+          dq += t * t;
         }
         for (int k = 1; k < gv; k <<= 1) {
           ds += __shfl_xor(ds, k);
           dq += __shfl_xor(dq, k);
         }
-        const double2 mm = moments_of(ds, dq, double(n.channels / n.groups), n.eps);
+        const double2 mm = moments_of(ds, dq, double(n.channels / n.groups), n.eps, double(m));
         if (near) {
 #pragma unroll
           for (int j = 0; j < V; ++j)
@@ -627,7 +639,7 @@ __global__ void __launch_bounds__(kRowThreads) k_rows(const Norm n) {
 // ---------------------------------------------------------------------------
 constexpr int kTileThreads = 256;
 
-// column sums of a tile: forward [slot][vecs] of x and x^2, backward [slot][channels] of dz and
+// column sums of a tile: forward [slot][vecs] of x - c and (x - c)^2, backward [slot][channels] of dz and
 // dz xhat; ragged tiles have two slots, an unused one is 0.  (These kernels are kept small: the
 // first wave of a CU waits about 0.1 us for every 64 bytes of its instructions, which for a few
 // MB of rows is most of the time.)
@@ -708,7 +720,7 @@ __device__ __forceinline__ void do_sums(const Norm& n, int64_t t, double2* red) 
       if (BWD) {
         fold();
       } else {
-        const double2 v = t1.sums();
+        const double2 v = t1.sums(base_of<T>(n, p.seg, p.start, col / gv));
         a[0] = v.x;
         b[0] = v.y;
       }
@@ -832,7 +844,7 @@ __global__ void __launch_bounds__(kJoinThreads) k_join(const Norm n, int64_t job
     if (BWD) {
       n.mom[job] = {v.x / total, v.y / total};
     } else {
-      const double2 m = moments_of(v.x, v.y, total, n.eps);
+      const double2 m = moments_of(v.x, v.y, total, n.eps, base_of<T>(n, s, r0, g));
       n.stats[2 * job] = m.x;
       n.stats[2 * job + 1] = m.y;
     }

@@ -428,3 +428,26 @@ def test_an_eps_of_zero(shape, act):
     for dtype in (torch.float32, torch.bfloat16):
         check(data(shape, dtype), C // 8 if C % 8 == 0 else 3, *affine(C, torch.float32), act=act, eps=0.0)
         check(data(shape, dtype), C // 8 if C % 8 == 0 else 3, *affine(C, torch.float32), act=act, eps=1e-60)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("level", [2.0 ** 17, 2.0 ** 20, -2.0 ** 22])
+@pytest.mark.parametrize("act", ["none", "relu"])
+def test_levels_far_above_the_spread(level, act):
+    """Up to where a step of fp32 is a third of the spread: rows, groups of three of a row, short
+    and long dense segments, ragged ones of both kinds."""
+    for shape, groups in (((300, 64), 8), ((64, 24), 8), ((5, 30, 24), 4), ((3, 4000, 24), 4)):
+        check(data(shape, torch.float32, level=level), groups, *affine(shape[-1], torch.float32), act=act)
+    lens = [3, 0, 40, 700, 1, 31]
+    check(data((780, 24), torch.float32, level=level), 4, *affine(24, torch.float32), act=act, lens=lens,
+          ptr=torch.tensor([0] + lens).cumsum(0).to(DEV))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("shape", [(40, 24), (5, 30, 24), (3, 4000, 24)])
+def test_a_constant_far_from_zero(shape):
+    """Its variance is 0, not what squares of it would leave: the output is the bias, the gradient
+    1 / sqrt(eps) times the centred w dy."""
+    x = torch.full(shape, 1e6, device=DEV)
+    y = check(x, 8, *affine(24, torch.float32))
+    assert torch.equal(y.detach(), affine(24, torch.float32)[1].expand(shape))
