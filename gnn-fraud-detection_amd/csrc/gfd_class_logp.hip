@@ -9,10 +9,10 @@
 // again and writes its gradient.  16-bit logits leave about 14 vector
 // operations for an element at the card's copy rate, and the sums take ten (an
 // exponential counts four), so the loop is kept to them:
-//   * R is any reference not far below the row's largest logit, not that logit:
-//     a lane moves its own only when a logit exceeds it by more than kSlack.  A
+//   * R is, while a row is read, any reference not far below its largest logit: a
+//     lane moves its own only when a logit exceeds it by more than kSlack.  A
 //     running maximum would be moved by one of the 64 lanes in nearly every
-//     iteration.
+//     iteration.  The lanes' sums are joined about the largest logit.
 //   * The top list is a wave's: entry j in lane j.  A vector of logits enters the
 //     search only where its largest is above the list's last entry, the same
 //     comparison as the reference's; the waves that share a row tell each other
@@ -108,9 +108,9 @@ struct Sums {
     s += e;
     t = fmaf(e, max_f(d, -1000.f), t);  // e = 0 at d = -inf: adds 0
   }
-  // the wave's sums, in every lane of it
-  __device__ __forceinline__ void join() {
-    const float to = wave_max(r);
+  // the wave's sums about its largest logit, in every lane of it; ``most``: the lane's
+  __device__ __forceinline__ void join(float most) {
+    const float to = wave_max(most);
     if (to != -kInf) move(to);
     s = wave_sum(s);
     t = wave_sum(t);
@@ -360,12 +360,12 @@ struct Partial {  // of a wave or a split
   float r, s, t;
 };
 
-// sums and top list of the elements [begin, end) of a row that this wave reads:
+// sums, largest logit and top list of the elements [begin, end) of a row that this wave reads:
 // wave w of W.  best_floor (LDS, nullable): the highest floor of the waves' lists, a bound
 // from below of the row's list
 template <typename T, int W>
 __device__ __forceinline__ void scan_row(const T* xr, int begin, int end, int w, int top, Sums& a,
-                                         Top& best, volatile float* best_floor) {
+                                         float& most, Top& best, volatile float* best_floor) {
   constexpr int V = 16 / sizeof(T);
   constexpr int U = 2;  // vectors in flight a lane
   const int lane = threadIdx.x & 63;
@@ -423,6 +423,7 @@ __device__ __forceinline__ void scan_row(const T* xr, int begin, int end, int w,
       for (int j = 0; j < V; j += 2) m[u] = max3_f(m[u], to_f32(q[u].v[j]), to_f32(q[u].v[j + 1]));
       all = max_f(all, m[u]);
     }
+    most = max_f(most, all);
     if (__ballot(all > bound) || (top && (last || best.size < top))) {
       if (all > a.r + kSlack) a.move(all);
       if (top) {
@@ -505,8 +506,9 @@ __global__ void __launch_bounds__(kThreads, 8) k_fwd_wide(const T* __restrict__ 
     }
     Sums a;
     Top best;
-    scan_row<T, W>(xr, begin, end, W > 1 ? wave : 0, top, a, best, &best_floor);
-    a.join();
+    float most = -kInf;
+    scan_row<T, W>(xr, begin, end, W > 1 ? wave : 0, top, a, most, best, &best_floor);
+    a.join(most);
     if (W > 1) {
       if (lane == 0) sums[wave] = {a.r, a.s, a.t};
       if (wave > 0 && lane < top) lists[wave * top + lane] = {best.val, best.cls};
@@ -518,7 +520,7 @@ __global__ void __launch_bounds__(kThreads, 8) k_fwd_wide(const T* __restrict__ 
           a.s = sums[lane].s;
           a.t = sums[lane].t;
         }
-        a.join();
+        a.join(a.r);
         if (top) {
           for (int w = 1; w < W; ++w) {
             Entry e = {__builtin_nanf(""), 0};
@@ -589,7 +591,7 @@ __global__ void __launch_bounds__(kWave) k_fwd_join(const T* __restrict__ x, int
         if (top) head = max_f(head, from[i * top + level].val);
       }
     }
-    a.join();
+    a.join(a.r);
     if (lane == 0) write_row(o, row, given, a.r, a.s, a.t);
     if (top) {
       const float least = Top::bound_of(head, need);

@@ -357,3 +357,28 @@ def test_c_argument_errors():
     assert fwd(x=None) == 1 and fwd(x=258) == 1 and fwd(target=None) == 1 and fwd(ent=None) == 1
     assert fwd(top=2, tc=None) == 1 and fwd(stats=None) == 1
     assert fwd(classes=200000) == 3                            # no workspace
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("V", [20, 130, 700, 5000, 70001])
+@pytest.mark.parametrize("N", [3, 1500])
+def test_statistics_are_the_maximum_and_the_log_sum(N, V):
+    """As include/gfd.h states them, also of a row whose largest logit follows some that lie less
+    than its sums' slack below it, and of a confident one; log probabilities are not above 0,
+    entropies not below it."""
+    from gfd import fused
+    x = torch.full((N, V), -50.0)
+    x[:, ::2] = 0.0
+    x[:, V // 2 + 1::max(V // 5, 1)] = 7.5
+    x[1] = -90.0
+    x[1, V - 1] = 12.25
+    x[2] = torch.randn(V, generator=torch.Generator().manual_seed(2)) * 3
+    t = x.argmax(1)
+    m = x.double().amax(1)
+    ls = (x.double() - m[:, None]).exp().sum(1).log()
+    for top in (0, 3):
+        logp, entropy, top_logp, _, stats = fused._class_log_probs_fwd(x.to(DEV), t.to(DEV), top, -1, True)
+        assert torch.equal(stats[:, 0].cpu().double(), m)
+        # a sum's roundings, and those of exponents up to 16 in it
+        assert ((stats[:, 1].cpu().double() - ls).abs() <= U * (64 + V / 64)).all()
+        assert (logp <= 0).all() and (entropy >= 0).all() and (top_logp <= 0).all()
