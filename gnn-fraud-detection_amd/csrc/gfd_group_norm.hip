@@ -60,7 +60,6 @@ struct Norm {
   int part0;       // first row of ``part`` that the teams write (backward)
   int cols, rows;  // threads over a row's vectors and over rows, powers of two
   int cols2, rows2;  // their logarithms
-  int zero_rest;   // ragged: k_apply clears the rows of no segment
 };
 
 // ---------------------------------------------------------------------------
