@@ -916,7 +916,7 @@ def all_reduce_grads(params, group=None) -> None:
     # the flat buffers then line up element for element
     flat = torch.cat([(p.grad if p.grad is not None else torch.zeros_like(p)).reshape(-1)
                       for p in ps])
-    dist.all_reduce(flat, group=group)
+    _all_reduce(flat, group)
     off = 0
     for p in ps:
         n = p.numel()
@@ -961,6 +961,8 @@ def _a2a(out: torch.Tensor, inp: torch.Tensor, out_splits, in_splits, group) -> 
 
 
 def _all_reduce(t: torch.Tensor, group) -> None:
+    """Sum of ``t`` over the ranks, in place; device tensors over gloo are staged
+    through host memory."""
     import torch.distributed as dist
     if t.is_cuda and dist.get_backend(group) == "gloo":
         h = t.cpu()

@@ -289,3 +289,31 @@ def test_all_reduce_grads_missing_grads_and_bn_without_affine():
     for rank in (0, 1):
         assert torch.allclose(res[rank][3], bn.running_mean, atol=1e-12)
         assert torch.allclose(res[rank][4], bn.running_var, atol=1e-12)
+
+
+class _OnADevice(torch.Tensor):
+    """A tensor that says it is on a GPU, as far as collectives look."""
+    is_cuda = True
+
+    def cpu(self):
+        return self.as_subclass(torch.Tensor).clone()
+
+
+def test_gradients_of_a_device_are_staged_for_gloo(monkeypatch):
+    """gloo gets tensors of the host alone; the sum comes back to the device's gradients."""
+    import torch.distributed as dist
+    from gfd import dist as gdist
+    seen = []
+
+    def all_reduce(t, op=None, group=None):
+        seen.append(t.is_cuda)
+        t.mul_(2)
+
+    monkeypatch.setattr(dist, "get_world_size", lambda group=None: 2)
+    monkeypatch.setattr(dist, "get_backend", lambda group=None: "gloo")
+    monkeypatch.setattr(dist, "all_reduce", all_reduce)
+    params = [torch.zeros(n).as_subclass(_OnADevice).requires_grad_() for n in (5, 3)]
+    params[0].grad = torch.ones(5).as_subclass(_OnADevice)
+    gdist.all_reduce_grads(params)
+    assert seen == [False]
+    assert params[0].grad.tolist() == [2.0] * 5 and params[1].grad.tolist() == [0.0] * 3
