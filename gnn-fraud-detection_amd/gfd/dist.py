@@ -1096,11 +1096,13 @@ def gat_forward_sharded_train(model, x: torch.Tensor, local: LocalGraph, plan: H
         if getattr(model, "group_norms", None) is not None:
             # a node's own statistics: nothing to exchange (the relu is the norm's)
             y = model.group_norms[li](y)
-        elif model.batch_norms is not None:
-            bn = model.batch_norms[li]
-            # eval: the running statistics, identical on every rank
-            y = sharded_batch_norm(y, bn, n_total, group) if model.training else bn(y)
-        y = F.dropout(F.relu(y), p=model.dropout, training=model.training)
+        else:
+            if model.batch_norms is not None:
+                bn = model.batch_norms[li]
+                # eval: the running statistics, identical on every rank
+                y = sharded_batch_norm(y, bn, n_total, group) if model.training else bn(y)
+            y = F.relu(y)
+        y = F.dropout(y, p=model.dropout, training=model.training)
         h_prev = x_local[:local.n_dst]
         h_own = h_prev + y if (model.residual and h_prev.size(-1) == y.size(-1)) else y
     return _head(model.out, h_own)

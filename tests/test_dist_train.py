@@ -317,3 +317,24 @@ def test_gradients_of_a_device_are_staged_for_gloo(monkeypatch):
     gdist.all_reduce_grads(params)
     assert seen == [False]
     assert params[0].grad.tolist() == [2.0] * 5 and params[1].grad.tolist() == [0.0] * 3
+
+
+@pytest.mark.parametrize("norm", ["group", "batch", "none"])
+def test_one_relu_a_layer(monkeypatch, norm):
+    """A group norm applies it itself; behind a BatchNorm, or no norm, it is a pass of its own."""
+    import types
+
+    import torch.nn.functional as Fn
+    from gfd import models
+    m = models.GAT(6, 64, 2, num_layers=1, dropout=0.0, use_batch_norm=norm == "batch",
+                   norm="group" if norm == "group" else "batch").eval()
+    if norm == "group":
+        m.group_norms = torch.nn.ModuleList([torch.nn.Sequential(torch.nn.GroupNorm(8, 64), torch.nn.ReLU())])
+    rows, relu = torch.randn(9, 64), Fn.relu
+    seen = []
+    monkeypatch.setattr(Fn, "relu", lambda t, inplace=False: seen.append(1) or relu(t))
+    local = types.SimpleNamespace(lo=0, n_dst=9, rows=lambda x: x)
+    out = gdist.gat_forward_sharded_train(m, torch.randn(9, 6), local, None, 9, conv_fn=lambda *a: rows)
+    assert len(seen) == 1
+    y = rows if norm == "none" else (m.group_norms if norm == "group" else m.batch_norms)[0](rows)
+    assert torch.equal(out, m.out(relu(y)))
