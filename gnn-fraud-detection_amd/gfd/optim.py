@@ -128,11 +128,19 @@ class Adam(torch.optim.Optimizer):
         if torch.cuda.is_current_stream_capturing():
             raise RuntimeError("gfd Adam: call step() once before capturing it (the states are "
                                "made by the first call)")
+        f = self._flat[gi] = self._buffers(params, self.param_groups[gi]["state_bits"], dev)
+        for i, p in enumerate(params):
+            self.state[p] = self._views(f, i, p)
+        return f
+
+    @staticmethod
+    def _buffers(params: list, bits: int, dev) -> dict:
         first, total = [], 0
         for p in params:
             first.append(total)
             total += -(-p.numel() // STATE_BLOCK) * STATE_BLOCK
-        f = {"first": first, "numel": [p.numel() for p in params], "bits": self.param_groups[gi]["state_bits"], "device": dev,
+        total = max(total, STATE_BLOCK)          # of parameters without elements too there is a buffer
+        f = {"first": first, "numel": [p.numel() for p in params], "bits": bits, "device": dev,
              "step": torch.zeros(len(params), dtype=torch.int32, device=dev),
              "ticket": torch.zeros(1056, dtype=torch.int32, device=dev)}
         if f["bits"] == 32:
@@ -145,9 +153,6 @@ class Adam(torch.optim.Optimizer):
         # gfd_adam_tensor of every parameter; the two pointers are filled in at each step
         f["table"] = np.array([(0, 0, p.numel(), at, i) for i, (p, at) in enumerate(zip(params, first))],
                               dtype=np.int64)
-        self._flat[gi] = f
-        for i, p in enumerate(params):
-            self.state[p] = self._views(f, i, p)
         return f
 
     @staticmethod

@@ -530,7 +530,6 @@ def _on_the_host(monkeypatch, params, **kw):
     """An Adam over CPU parameters whose states are there and whose launches do nothing."""
     import types
 
-    import numpy as np
     from gfd import _lib, optim
     calls = _Written()
     for name in ("call", "call_on"):
@@ -538,14 +537,8 @@ def _on_the_host(monkeypatch, params, **kw):
     monkeypatch.setattr(_lib, "load", lambda: calls)
     monkeypatch.setattr(_lib, "stream_handle", lambda device=None: 0)
     opt = optim.Adam(params, **kw)
-    first = [0]
-    for p in params:
-        first.append(first[-1] + -(-p.numel() // BLOCK) * BLOCK)
-    f = {"first": first[:-1], "numel": [p.numel() for p in params], "bits": 32,
-         "device": types.SimpleNamespace(index=-1), "step": torch.zeros(len(params), dtype=torch.int32),
-         "ticket": torch.zeros(1056, dtype=torch.int32), "exp_avg": torch.zeros(first[-1]),
-         "exp_avg_sq": torch.zeros(first[-1]),
-         "table": np.array([(0, 0, p.numel(), at, i) for i, (p, at) in enumerate(zip(params, first))], dtype=np.int64)}
+    f = opt._buffers(params, 32, torch.device("cpu"))
+    f["device"] = types.SimpleNamespace(index=-1)
     opt._flat[0] = f
     for i, p in enumerate(params):
         opt.state[p] = opt._views(f, i, p)
@@ -686,3 +679,28 @@ def test_a_load_with_other_bits_makes_the_states_anew():
     opt.step()
     other.step()
     assert torch.equal(p, q)
+
+
+def test_parameters_without_elements_have_a_buffer():
+    """The library takes no null pointer for the states."""
+    from gfd.optim import Adam
+    for bits in (32, 8):
+        f = Adam._buffers([torch.zeros(0), torch.zeros(0, 4)], bits, torch.device("cpu"))
+        assert all(t.numel() and t.data_ptr() for t in f.values() if isinstance(t, torch.Tensor))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("bits", [32, 8])
+def test_a_group_without_elements_steps(bits):
+    from gfd.optim import Adam
+    p, q = make([0, (0, 3)], torch.float32)
+    r, = make([300], torch.float32)
+    before = r.detach().clone()
+    opt = Adam([{"params": [p, q]}, {"params": [r]}], lr=0.1, state_bits=bits)
+    for _ in range(2):
+        opt.step()
+    assert opt.state[p]["step"].item() == 2 and opt.state[q]["exp_avg"].shape == (0, 3)
+    assert not torch.equal(r, before)
+    opt.load_state_dict(copy.deepcopy(opt.state_dict()))
+    opt.step()
+    assert opt.state[q]["step"].item() == 3
