@@ -141,6 +141,8 @@ class Adam(torch.optim.Optimizer):
             total += -(-p.numel() // STATE_BLOCK) * STATE_BLOCK
         total = max(total, STATE_BLOCK)          # of parameters without elements too there is a buffer
         f = {"first": first, "numel": [p.numel() for p in params], "bits": bits, "device": dev,
+             # the strides that the states have too; None: contiguous
+             "strides": [None if p.is_contiguous() else p.stride() for p in params],
              "step": torch.zeros(len(params), dtype=torch.int32, device=dev),
              "ticket": torch.zeros(1056, dtype=torch.int32, device=dev)}
         if f["bits"] == 32:
@@ -289,7 +291,8 @@ class Adam(torch.optim.Optimizer):
                 list(map(_layout, grads)).count(torch.strided) == n and
                 list(map(_device, params)).count(index) == n == list(map(_device, grads)).count(index) and
                 list(map(_numel, params)) == numel == list(map(_numel, grads)) and
-                all(map(_contiguous, params)) and all(map(_contiguous, grads))):
+                all(map(_contiguous, params)) and all(map(_contiguous, grads)) and
+                f["strides"].count(None) == n):
             table = f["table"]
             table[:, 0] = list(map(_data_ptr, params))
             table[:, 1] = list(map(_data_ptr, grads))
@@ -321,6 +324,9 @@ class Adam(torch.optim.Optimizer):
             n = numel[i]
             if p.numel() != n or g.numel() != n:
                 raise RuntimeError(f"gfd Adam: a parameter changed its size from {n} to {p.numel()}")
+            if (None if p.is_contiguous() else p.stride()) != f["strides"][i]:
+                raise RuntimeError("gfd Adam: a parameter changed its strides to "
+                                   f"{p.stride()} after its states were made")
             if not (p.is_contiguous() and g.is_contiguous()) and g.stride() != p.stride():
                 g = torch.empty_like(p).copy_(g)
                 kept.append(g)
@@ -341,6 +347,8 @@ class Adam(torch.optim.Optimizer):
             if lr.device != dev:
                 raise RuntimeError(f"gfd Adam: lr is on {lr.device}, expected {dev}")
             lr, lr_ptr = 0.0, lr.data_ptr()
+        if dtype not in _CODES:
+            raise RuntimeError(f"gfd Adam: a parameter changed its type to {dtype}")
         b1, b2 = group["betas"]
         _check_apart(table, dtype.itemsize)
         _lib.call_on(dev, "gfd_adam_step", table.ctypes.data, len(table), _CODES[dtype], f["bits"],

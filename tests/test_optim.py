@@ -704,3 +704,24 @@ def test_a_group_without_elements_steps(bits):
     opt.load_state_dict(copy.deepcopy(opt.state_dict()))
     opt.step()
     assert opt.state[q]["step"].item() == 3
+
+
+def test_a_parameter_that_changes_after_its_states_were_made(monkeypatch):
+    """Other strides would take other elements' moments, or memory that is not the parameter's."""
+    p = torch.zeros((4, 6), requires_grad=True)
+    q = torch.zeros((6, 4)).t().requires_grad_()
+    p.grad, q.grad = torch.ones(4, 6), torch.ones(4, 6)
+    opt, calls = _on_the_host(monkeypatch, [p, q])
+    opt.step()
+    assert calls.calls == ["gfd_adam_step"]
+    for t, data in ((p, torch.zeros((6, 4)).t()), (p, torch.zeros((4, 12))[:, ::2]), (q, torch.zeros((4, 6))),
+                    (q, torch.zeros((6, 8)).t()[:4])):
+        was, t.data = t.data, data
+        with pytest.raises(RuntimeError, match="strides"):
+            opt.step()
+        t.data = was
+    for t in (p, q):
+        t.data, t.grad = t.data.double(), t.grad.double()
+    with pytest.raises(RuntimeError, match="type"):
+        opt.step()
+    assert calls.calls == ["gfd_adam_step"]
