@@ -4,7 +4,9 @@ in fp32 or in 8 bits.
 Drop-in for ``torch.optim.Adam(model.parameters(), lr=0.001,
 weight_decay=5e-4)`` of the reference's training loop (train.py:353, stepped at
 train.py:143): the same constructor arguments and update, over
-``gfd_adam_step``.
+``gfd_adam_step``.  ``amsgrad``, ``maximize`` and ``differentiable`` can only be
+false; ``foreach``, ``capturable`` and ``fused``, which choose among torch's own
+implementations, change nothing.
 
 * ``state_bits=32``: the two moments in fp32.  ``state_bits=8``: the first
   moment and the root of the second as e4m3 codes over a power-of-two scale per
@@ -49,13 +51,22 @@ def _dense(p: torch.Tensor) -> bool:
     return p.is_contiguous() or torch.empty_like(p, device="meta").stride() == p.stride()
 
 
+def _refuse(options: dict) -> None:
+    for name in ("amsgrad", "maximize", "differentiable"):
+        if options.get(name):
+            raise NotImplementedError(f"gfd Adam: {name} is not supported")
+
+
 class Adam(torch.optim.Optimizer):
     """``torch.optim.Adam`` (weight decay added to the gradient)."""
 
     _decoupled = False
 
     def __init__(self, params, lr=1e-3, betas=(0.9, 0.999), eps: float = 1e-8,
-                 weight_decay: float = 0.0, *, state_bits: int = 32, seed: int = 0):
+                 weight_decay: float = 0.0, amsgrad: bool = False, *, foreach=None,
+                 maximize: bool = False, capturable: bool = False, differentiable: bool = False,
+                 fused=None, state_bits: int = 32, seed: int = 0):
+        _refuse(dict(amsgrad=amsgrad, maximize=maximize, differentiable=differentiable))
         self._flat: Dict[int, dict] = {}
         super().__init__(params, dict(lr=lr, betas=tuple(betas), eps=eps,
                                       weight_decay=weight_decay, state_bits=state_bits, seed=seed,
@@ -86,9 +97,7 @@ class Adam(torch.optim.Optimizer):
             raise ValueError(f"gfd Adam: state_bits is 32 or 8 (got {group['state_bits']})")
         if not 0 <= int(group["seed"]) < 2 ** 32:
             raise ValueError(f"gfd Adam: seed must be in [0, 2**32) (got {group['seed']})")
-        for other in ("amsgrad", "maximize"):
-            if group.get(other):
-                raise NotImplementedError(f"gfd Adam: {other} is not supported")
+        _refuse(group)
         if group["decoupled_weight_decay"] != self._decoupled:
             raise ValueError("gfd Adam: Adam adds the weight decay to the gradient, AdamW applies it to "
                              "the parameter; a group is of the other kind")
@@ -376,5 +385,5 @@ class AdamW(Adam):
     _decoupled = True
 
     def __init__(self, params, lr=1e-3, betas=(0.9, 0.999), eps: float = 1e-8,
-                 weight_decay: float = 1e-2, *, state_bits: int = 32, seed: int = 0):
-        super().__init__(params, lr, betas, eps, weight_decay, state_bits=state_bits, seed=seed)
+                 weight_decay: float = 1e-2, amsgrad: bool = False, **options):
+        super().__init__(params, lr, betas, eps, weight_decay, amsgrad, **options)

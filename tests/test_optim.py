@@ -725,3 +725,22 @@ def test_a_parameter_that_changes_after_its_states_were_made(monkeypatch):
     with pytest.raises(RuntimeError, match="type"):
         opt.step()
     assert calls.calls == ["gfd_adam_step"]
+
+
+def test_the_options_of_torch():
+    """torch's constructor calls: what changes the rule is refused, what chooses an implementation
+    taken."""
+    from gfd.optim import Adam, AdamW
+    p = torch.zeros(4, requires_grad=True)
+    for cls in (Adam, AdamW):
+        opt = cls([p], 1e-2, (0.8, 0.9), 1e-6, 0.1, False, foreach=True, maximize=False, capturable=True,
+                  differentiable=False, fused=None, state_bits=8, seed=3)
+        group = opt.param_groups[0]
+        assert (group["lr"], group["weight_decay"], group["state_bits"], group["seed"]) == (1e-2, 0.1, 8, 3)
+        for name in ("amsgrad", "maximize", "differentiable"):
+            with pytest.raises(NotImplementedError, match=name):
+                cls([p], **{name: True})
+            with pytest.raises(NotImplementedError, match=name):
+                cls([{"params": [p], name: True}])
+        with pytest.raises(TypeError):
+            cls([p], decay=1.0)
