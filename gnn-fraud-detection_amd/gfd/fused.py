@@ -336,6 +336,8 @@ class _BNReluDropout(torch.autograd.Function):
                   _lib.ptr(rv), 1 if relu else 0, float(p), seed, out.data_ptr(),
                   mean.data_ptr(), invstd.data_ptr(), ws.data_ptr(), ws.numel(),
                   _lib.stream_handle(dev))
+        if rm is not None:                      # written by the call: what eval_weights goes by
+            torch.autograd.graph.increment_version([rm, rv])
         ctx.save_for_backward(y, gamma, beta, mean, invstd)
         ctx.relu, ctx.p, ctx.seed, ctx.has_res = relu, p, seed, res is not None
         return out

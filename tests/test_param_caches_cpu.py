@@ -78,3 +78,20 @@ def test_x_colmax_is_kept_per_tensor_object_and_version(monkeypatch):
         gnn.x_colmax(torch.randn(3, 7))
     assert len(gnn._COLMAX) <= gnn._COLMAX_ENTRIES
     gnn._COLMAX.clear()
+
+
+def test_a_training_pass_raises_the_versions_of_the_running_statistics(monkeypatch):
+    """They are written through their addresses; evaluation after a training-mode pass without a
+    step (new statistics for frozen weights) folds the new ones."""
+    stub = _patch(monkeypatch)
+    stub.gfd_bn_workspace_size = lambda: 16
+    conv = gnn.GATConv(16, 64, heads=8, concat=False)
+    bn = torch.nn.BatchNorm1d(64)
+    dev = torch.device("cpu")
+    _, a1 = fused.eval_weights(conv, bn, dev)
+    fused.train_body(torch.randn(5, 64), bn.train(), None)
+    assert stub.calls.count("gfd_bn_relu_fwd") == 1
+    _, a2 = fused.eval_weights(conv, bn, dev)
+    assert a2 is not a1
+    assert fused.eval_weights(conv, bn, dev)[1] is a2
+    fused.train_body(torch.randn(5, 64), torch.nn.BatchNorm1d(64, track_running_stats=False), None)

@@ -432,3 +432,22 @@ def test_offloaded_and_checkpointed_passes_give_the_same_gradients():
             # another alignment is another order of a row's fp32 sums: 48 roundings, for each of
             # the three passes
             assert_close_scaled(a, b, rtol=3 * 48 * 2.0 ** -24)
+
+
+@pytest.mark.gpu
+def test_evaluation_follows_new_running_statistics():
+    """A training-mode pass without a step between two evaluations."""
+    from gfd import models
+    ei, x, _ = (t.to(DEV) for t in _problem())
+
+    def make():
+        torch.manual_seed(3)
+        return models.GAT(WIDTH, 64, 1, num_layers=2, dropout=0.0).to(DEV)
+
+    m, fresh = make(), make()
+    with torch.no_grad():
+        before = m.eval()(x, ei)
+        m.train()(x * 3, ei)
+        fresh.load_state_dict(m.state_dict())
+        after = m.eval()(x, ei)
+        assert torch.equal(after, fresh.eval()(x, ei)) and not torch.equal(after, before)
