@@ -946,10 +946,10 @@ struct Cut {
 
 Cut cut_of(int64_t segments, int64_t length, bool ragged, int channels) {
   Cut c;
-  const int64_t rows = ragged ? length : segments * length;
-  // tiles: about 1024 of them, 32 to 512 rows
-  int64_t tile = pow2_up((rows + 1023) / 1024);
-  tile = tile < 32 ? 32 : tile > 512 ? 512 : tile;
+  // tiles: about 1024 of them, 32 to 512 rows (more dense segments than kMaxTiled have none)
+  const int64_t rows = ragged ? length : segments <= kMaxTiled ? segments * length : 0;
+  int64_t tile = rows < 512 * 1024 ? pow2_up((rows + 1023) / 1024) : 512;
+  tile = tile < 32 ? 32 : tile;
   c.tile = int(tile);
   if (ragged) {
     c.team = c.tiled = true;

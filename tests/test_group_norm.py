@@ -451,3 +451,17 @@ def test_a_constant_far_from_zero(shape):
     x = torch.full(shape, 1e6, device=DEV)
     y = check(x, 8, *affine(24, torch.float32))
     assert torch.equal(y.detach(), affine(24, torch.float32)[1].expand(shape))
+
+
+def test_workspace_of_the_largest_shapes():
+    """Sizes whose rows leave 31 or 63 bits are answered, and a call with more tiles than a launch
+    counts is refused."""
+    from gfd import _lib
+    lib = _lib.load()
+    for segments, length in ((2, 1 << 40), (65535, 1 << 40), (1 << 40, 1 << 40), (65536, 1 << 40)):
+        for backward in (0, 1):
+            assert lib.gfd_group_norm_workspace_size(segments, length, 0, 64, 8, backward) >= 0
+    assert lib.gfd_group_norm_workspace_size(2, 1 << 40, 1, 64, 8, 1) > 0
+    for ptr in (None, 256):
+        assert lib.gfd_group_norm_fwd(256, 0, 2, 1 << 40, ptr, 64, 8, 64, 0, None, None, 0, 1e-5, 0, 256, None,
+                                      None, 0, None) == 5
