@@ -167,29 +167,37 @@ __device__ __forceinline__ float less(float a, float b, float c) {
   return a * b - c;
 }
 
-// activation and, where d is not null, its derivative at z
-template <int ACT>
+// activation and, where d is not null, its derivative at z.  WIDE: of fp32 rows
+template <int ACT, bool WIDE>
 __device__ __forceinline__ float activate(float z, float* d) {
   switch (ACT) {
     case GFD_ACT_RELU:
       if (d) *d = z > 0.f ? 1.f : 0.f;
       return z > 0.f ? z : z != z ? z : 0.f;
     case GFD_ACT_SILU: {
+      // (v_rcp_f32 and the exponential are within 2^-23 of themselves, as two roundings are)
       const float p = __builtin_amdgcn_rcpf(1.f + exp_of(-z));
       if (d) *d = p * (1.f + z * (1.f - p));
       return z * p;
     }
     case GFD_ACT_GELU: {
-      // Phi(z) = (1 + erf(z / sqrt 2)) / 2 with Abramowitz and Stegun's 7.1.26: the tail
-      // e^(-z^2 / 2) times a polynomial in 1 / (1 + p |z| / sqrt 2), within 7.5e-8; its
-      // exponential is the derivative's too
       const float e = exp_of(-0.5f * z * z);
-      const float t = __builtin_amdgcn_rcpf(fmaf(fabsf(z), 0.3275911f * 0.70710678118654752f, 1.f));
-      float q = fmaf(t, 0.5f * 1.061405429f, 0.5f * -1.453152027f);
-      q = fmaf(t, q, 0.5f * 1.421413741f);
-      q = fmaf(t, q, 0.5f * -0.284496736f);
-      q = fmaf(t, q, 0.5f * 0.254829592f) * t * e;
-      const float p = z > 0.f ? 1.f - q : q;
+      float p;  // Phi(z)
+      if constexpr (WIDE) {
+        p = fmaf(0.5f, erff(z * 0.70710678118654752f), 0.5f);
+      } else {
+        // Phi(-|z|) = e^(-z^2 / 2) times a polynomial in t = 1 / (1 + |z| / 4), fitted over 0 <=
+        // |z| <= 14 so that Phi is within 4e-9 and its tail within 4e-5 of itself, a sixth of
+        // half a step of fp16; its exponential is the derivative's too
+        const float t = __builtin_amdgcn_rcpf(fmaf(fabsf(z), 0.25f, 1.f));
+        float q = fmaf(t, -0.0918481424f, 0.342620730f);
+        q = fmaf(t, q, -0.268634528f);
+        q = fmaf(t, q, 0.282492280f);
+        q = fmaf(t, q, 0.0242558978f);
+        q = fmaf(t, q, 0.112302706f);
+        q = fmaf(t, q, 0.0988110527f) * t * e;
+        p = z > 0.f ? 1.f - q : q;
+      }
       if (d) *d = fmaf(z * e, 0.39894228040143268f, p);
       return z * p;
     }
@@ -236,7 +244,7 @@ struct Columns {
 #pragma unroll
     for (int j = 0; j < V; ++j) {
       const float v = x.at(j);
-      y.v[j] = from_f32<T>(activate<ACT>(z(n, v, v - hi, j), nullptr));
+      y.v[j] = from_f32<T>(activate<ACT, sizeof(T) == 4>(z(n, v, v - hi, j), nullptr));
     }
     return y;
   }
@@ -248,7 +256,7 @@ struct Columns {
       const float v = x.at(j), d = v - hi;
       xh[j] = fmaf(d, r, -lr);
       float g;
-      activate<ACT>(z(n, v, d, j), &g);
+      activate<ACT, sizeof(T) == 4>(z(n, v, d, j), &g);
       dz[j] = dy.at(j) * g;
     }
   }
@@ -597,7 +605,7 @@ __global__ void __launch_bounds__(kRowThreads) k_rows(const Norm n) {
 #pragma unroll
         for (int j = 0; j < V; ++j) {
           float g;
-          activate<ACT>(z[j], &g);
+          activate<ACT, sizeof(T) == 4>(z[j], &g);
           dz[j] = dy[u].at(j) * g;
           const float wd = w[j] * dz[j];
           sa += wd;
@@ -610,7 +618,7 @@ __global__ void __launch_bounds__(kRowThreads) k_rows(const Norm n) {
         for (int j = 0; j < V; ++j) o.v[j] = from_f32<T>(r * (less(w[j], dz[j], ma) - xh[j] * mb));
       } else {
 #pragma unroll
-        for (int j = 0; j < V; ++j) o.v[j] = from_f32<T>(activate<ACT>(z[j], nullptr));
+        for (int j = 0; j < V; ++j) o.v[j] = from_f32<T>(activate<ACT, sizeof(T) == 4>(z[j], nullptr));
       }
       if (on && r0 + u * step < n.segments)
         *reinterpret_cast<Pack<T, V>*>(po + (r0 + u * step) * n.channels) = o;
