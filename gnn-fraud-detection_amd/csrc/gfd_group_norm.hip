@@ -127,12 +127,12 @@ __device__ __forceinline__ const T* row_in(const Norm& n, const void* base, int6
                : p + seg * n.seg_stride + (r - seg * n.length) * n.row_stride;
 }
 
-// what the sums of a segment (with rows, the first one ``start``) and a group are taken about in
-// fp64: its first element.  However far from 0 the group lies, the sum of squares is at most its
+// what the sums of a segment (with rows, the first one ``start``) and the group whose first channel
+// is ch are taken about in fp64: its first element.  However far from 0 the group lies, the sum of squares is at most its
 // number of elements times the spread's, so that of 53 bits only as many go as that number has
 template <typename T>
-__device__ __forceinline__ double base_of(const Norm& n, int64_t seg, int64_t start, int group) {
-  return double(to_f32(row_in<T>(n, n.x, seg, start)[group * (n.channels / n.groups)]));
+__device__ __forceinline__ T base_of(const Norm& n, int64_t seg, int64_t start, int ch) {
+  return static_cast<const T*>(n.x)[(n.ptr ? start * n.row_stride : seg * n.seg_stride) + ch];
 }
 
 // ---------------------------------------------------------------------------
@@ -361,8 +361,7 @@ __device__ __forceinline__ void do_team(const Norm& n, uint32_t block, uint32_t 
       return v;
     };
     // sums over the rows by column (f(k, col, a, b) adds a thread's), then of each group, handed
-    // to done(segment, its first row, group, a, b, its number of elements) and left at its first
-    // column
+    // to done(a, b, its number of elements) and left at its first column
     auto reduce = [&](auto f, auto done) {
 #pragma unroll
       for (int k = 0; k < NC; ++k) {
@@ -392,17 +391,19 @@ __device__ __forceinline__ void do_team(const Norm& n, uint32_t block, uint32_t 
           a += cs[k].x;
           b += cs[k].y;
         }
-        cs[0] = done(s0 + tm, q0, g, a, b, double(q1 - q0) * (n.channels / n.groups));
+        cs[0] = done(a, b, double(q1 - q0) * (n.channels / n.groups));
       }
       __syncthreads();
     };
     Columns<T, V, ACT> cols[NC];
     float ra[NC] = {}, rb[NC] = {};
+    T base[NC];
     const bool kept = BWD && n.stats;  // the forward's moments; else they are found (again)
     if (!kept)
       reduce(
-          [&](int, int col, double& a, double& b) {
+          [&](int k, int col, double& a, double& b) {
             Shifted t;
+            base[k] = base_of<T>(n, seg, r0, col / gv * gv * V);
             for (int64_t r = r0 + tr; r < r1; r += n.rows) {
               const Raw<T, V> x = x_at(r, col);
               if (t.n == 0) t.k = x.at(0);
@@ -410,18 +411,11 @@ __device__ __forceinline__ void do_team(const Norm& n, uint32_t block, uint32_t 
               for (int j = 0; j < V; ++j) t.add(x.at(j));
               t.fold(V);
             }
-            const double2 v = t.sums(base_of<T>(n, seg, r0, col / gv));
+            const double2 v = t.sums(to_f32(base[k]));  // (converted here: nothing waits for it before)
             a = v.x;
             b = v.y;
           },
-          [&](int64_t s, int64_t start, int g, double a, double b, double count) {
-            const double2 m = moments_of(a, b, count, n.eps, base_of<T>(n, s, start, g));
-            if (!BWD && n.stats) {
-              n.stats[2 * (s * n.groups + g)] = m.x;
-              n.stats[2 * (s * n.groups + g) + 1] = m.y;
-            }
-            return m;
-          });
+          [&](double a, double b, double count) { return moments_of(a, b, count, n.eps, 0.0); });
 #pragma unroll
     for (int k = 0; k < NC; ++k) {
       const int col = c + k * n.cols;
@@ -431,7 +425,13 @@ __device__ __forceinline__ void do_team(const Norm& n, uint32_t block, uint32_t 
           cols[k].set(n, col, st[0], st[1]);
         } else {
           const double2 m = col_sum[team * vecs + col / gv * gv];
-          cols[k].set(n, col, m.x, m.y);
+          const double mean = double(to_f32(base[k])) + m.x;
+          cols[k].set(n, col, mean, m.y);
+          if (!BWD && n.stats && tr == 0 && col % gv == 0) {
+            double* st = n.stats + 2 * (seg * n.groups + col / gv);
+            st[0] = mean;
+            st[1] = m.y;
+          }
         }
       }
     }
@@ -454,7 +454,7 @@ __device__ __forceinline__ void do_team(const Norm& n, uint32_t block, uint32_t 
               b += double(sb);
             }
           },
-          [&](int64_t, int64_t, int, double a, double b, double count) { return double2{a / count, b / count}; });
+          [](double a, double b, double count) { return double2{a / count, b / count}; });
 #pragma unroll
       for (int k = 0; k < NC; ++k) {
         const int col = c + k * n.cols;
@@ -727,7 +727,7 @@ __device__ __forceinline__ void do_sums(const Norm& n, int64_t t, double2* red) 
       if (BWD) {
         fold();
       } else {
-        const double2 v = t1.sums(base_of<T>(n, p.seg, p.start, col / gv));
+        const double2 v = t1.sums(to_f32(base_of<T>(n, p.seg, p.start, col / gv * gv * V)));
         a[0] = v.x;
         b[0] = v.y;
       }
@@ -851,7 +851,7 @@ __global__ void __launch_bounds__(kJoinThreads) k_join(const Norm n, int64_t job
     if (BWD) {
       n.mom[job] = {v.x / total, v.y / total};
     } else {
-      const double2 m = moments_of(v.x, v.y, total, n.eps, base_of<T>(n, s, r0, g));
+      const double2 m = moments_of(v.x, v.y, total, n.eps, to_f32(base_of<T>(n, s, r0, g * per)));
       n.stats[2 * job] = m.x;
       n.stats[2 * job + 1] = m.y;
     }
