@@ -382,3 +382,26 @@ def test_statistics_are_the_maximum_and_the_log_sum(N, V):
         # a sum's roundings, and those of exponents up to 16 in it
         assert ((stats[:, 1].cpu().double() - ls).abs() <= U * (64 + V / 64)).all()
         assert (logp <= 0).all() and (entropy >= 0).all() and (top_logp <= 0).all()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("N", [1, 2, 33])
+@pytest.mark.parametrize("V", [20, 700, 70001, 300000])
+def test_served(N, V):
+    """Without gradients (no statistics kept, the split rows' beside the partial lists): the
+    reference's values, and those with gradients to the bit."""
+    from gfd.fused import class_log_probs
+    x = logits(N, V, torch.bfloat16, seed=N)
+    for target, top in ((targets(N, V), 0), (targets(N, V), 7), (None, 0), (None, 64 if V > 64 else 3)):
+        with torch.no_grad():
+            r = class_log_probs(x, target, top)
+        logp, _, h, given, order = reference(x, target, top)
+        base = U * (64 + V / 64)
+        assert torch.equal(r.top_classes.cpu(), order)
+        want = logp.gather(1, order)
+        same(r.top_log_probs, want, base + 4 * U * want.abs(), "top")
+        same(r.entropy, h, base * (10 + h), "entropy")
+        if target is not None:
+            same(r.log_prob, given, base + 4 * U * given.abs(), "given")
+        for a, b in zip(r, class_log_probs(x.detach().requires_grad_(), target, top)):
+            assert a is b is None or torch.equal(a, b) and not a.requires_grad

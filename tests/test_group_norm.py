@@ -493,3 +493,22 @@ def test_gelu_to_its_type(dtype):
         assert (err <= 1.1 * torch.finfo(dtype).eps / 2 * want.abs().clamp(min=tiny)).all()
     # the sum of three, halved twice: 3 roundings more
     assert ((db.cpu().double() * 4 / 3 - slope).abs() <= 8 * U).all()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_served(dtype):
+    """Without gradients (the tiles' statistics go through the workspace): the formula's values,
+    and those with gradients to the bit, of rows, short and long dense segments, and a ragged
+    batch of both."""
+    from gfd.fused import group_norm
+    lens = [3, 0, 40, 2000, 1, 31, 700]
+    ptr = torch.tensor([0] + lens).cumsum(0).to(DEV)
+    w, b = affine(24, torch.float32)
+    for shape, at in (((300, 24), None), ((9, 40, 24), None), ((2, 3000, 24), None), ((sum(lens) + 3, 24), ptr)):
+        x = data(shape, dtype)
+        with torch.no_grad():
+            y = group_norm(x, 4, w, b, act="silu", ptr=at)
+        ry, size = reference(x, 4, w, b, 1e-5, "silu", lens if at is not None else None)
+        assert ((y.cpu().double() - ry).abs() <= OPS * size + half_step(dtype) * ry.abs()).all()
+        assert torch.equal(y, group_norm(x, 4, w.detach().requires_grad_(), b, act="silu", ptr=at))
