@@ -396,30 +396,31 @@ def _check_rows(what: str, name: str, t: torch.Tensor) -> None:
         raise TypeError(f"gfd {what}: {name} must be float32, bfloat16 or float16 (got {t.dtype})")
 
 
-def _norm_geometry(x, weight, bias, ptr, groups) -> tuple:
-    """The shape arguments of the group norm's C calls: (before the affine tensors, GFD_DTYPE_* of
-    these)."""
-    segments, length = (ptr.numel() - 1, x.size(0)) if ptr is not None else (x.size(0), x.size(1))
-    w_dtype = weight.dtype if weight is not None else bias.dtype if bias is not None else x.dtype
-    return ((_ROW_DTYPES[x.dtype], segments, length, _lib.ptr(ptr), x.size(-1), groups, x.stride(-2),
-             0 if ptr is not None else x.stride(0)), _ROW_DTYPES[w_dtype])
+def _norm_shape(x, ptr, groups) -> tuple:
+    """The arguments of the group norm's C calls that say how x lies."""
+    ragged = ptr is not None
+    segments, length = (ptr.numel() - 1, x.size(0)) if ragged else (x.size(0), x.size(1))
+    return (_ROW_DTYPES[x.dtype], segments, length, _lib.ptr(ptr), x.size(-1), groups, x.stride(-2),
+            0 if ragged else x.stride(0))
 
 
 def _group_norm_fwd(x, weight, bias, ptr, groups, eps, act, keep):
-    """(y, statistics or None)."""
-    dev, ragged, C = x.device, ptr is not None, x.size(-1)
-    geom, w_dtype = _norm_geometry(x, weight, bias, ptr, groups)
-    segments, length = geom[1:3]
+    """(y, statistics or None, _norm_shape's, GFD_DTYPE_* of the affine)."""
+    dev, ragged = x.device, ptr is not None
+    shape = _norm_shape(x, ptr, groups)
+    _, segments, length, _, C, _, _, _ = shape
     y = torch.empty(x.shape, dtype=x.dtype, device=dev)
     # a row of its own keeps no statistics: the backward finds them again
     stats = (torch.empty((segments, groups, 2), dtype=torch.float64, device=dev)
              if keep and (ragged or length != 1) else None)
+    w_dtype = _ROW_DTYPES[weight.dtype if weight is not None else
+                          bias.dtype if bias is not None else x.dtype]
     nbytes = _lib.load().gfd_group_norm_workspace_size(segments, length, int(ragged), C, groups, 0)
     ws = _ws(nbytes, dev) if nbytes else None
-    _lib.call_on(dev, "gfd_group_norm_fwd", x.data_ptr(), *geom, _lib.ptr(weight), _lib.ptr(bias),
+    _lib.call_on(dev, "gfd_group_norm_fwd", x.data_ptr(), *shape, _lib.ptr(weight), _lib.ptr(bias),
                  w_dtype, eps, act, y.data_ptr(), _lib.ptr(stats), _lib.ptr(ws), nbytes,
                  _lib.stream_handle(dev))
-    return y, stats
+    return y, stats, shape, w_dtype
 
 
 class _GroupNorm(torch.autograd.Function):
@@ -429,32 +430,43 @@ class _GroupNorm(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx, x, weight, bias, ptr, groups, eps, act):
-        y, stats = _group_norm_fwd(x, weight, bias, ptr, groups, eps, act, True)
+        y, stats, ctx.shape, ctx.w_dtype = _group_norm_fwd(x, weight, bias, ptr, groups, eps, act, True)
         ctx.save_for_backward(x, weight, bias, ptr, stats)
-        ctx.groups, ctx.act, ctx.eps = groups, act, eps
+        ctx.act, ctx.eps, ctx.strides = act, eps, x.stride()
         return y
 
     @staticmethod
     @once_differentiable
     def backward(ctx, grad):
-        # saved-tensor hooks may bring them back elsewhere and in other strides
         x, weight, bias, ptr, stats = ctx.saved_tensors
-        x = _unit_rows(x)
-        weight, bias, ptr, stats = map(_packed, (weight, bias, ptr, stats))
+        shape = ctx.shape
+        _, segments, length, at, C, groups, _, _ = shape
+        if x.stride() != ctx.strides or at != _lib.ptr(ptr) or _gaps(weight, bias, ptr, stats):
+            # saved-tensor hooks brought them back elsewhere, or in other strides
+            x = _unit_rows(x)
+            weight, bias, ptr, stats = map(_packed, (weight, bias, ptr, stats))
+            shape = _norm_shape(x, ptr, groups)
         dev = x.device
         grad = grad.contiguous()
         gx = torch.empty(x.shape, dtype=x.dtype, device=dev)
         gw = torch.empty_like(weight) if weight is not None and ctx.needs_input_grad[1] else None
         gb = torch.empty_like(bias) if bias is not None and ctx.needs_input_grad[2] else None
-        geom, w_dtype = _norm_geometry(x, weight, bias, ptr, ctx.groups)
-        nbytes = _lib.load().gfd_group_norm_workspace_size(*geom[1:3], int(ptr is not None), x.size(-1),
-                                                           ctx.groups, 1)
+        nbytes = _lib.load().gfd_group_norm_workspace_size(segments, length, int(ptr is not None), C,
+                                                           groups, 1)
         ws = _ws(nbytes, dev)
-        _lib.call_on(dev, "gfd_group_norm_bwd", x.data_ptr(), *geom, _lib.ptr(weight),
-                     _lib.ptr(bias), w_dtype, ctx.eps, ctx.act, _lib.ptr(stats), grad.data_ptr(),
+        _lib.call_on(dev, "gfd_group_norm_bwd", x.data_ptr(), *shape, _lib.ptr(weight),
+                     _lib.ptr(bias), ctx.w_dtype, ctx.eps, ctx.act, _lib.ptr(stats), grad.data_ptr(),
                      gx.data_ptr(), _lib.ptr(gw), _lib.ptr(gb), ws.data_ptr(), ws.numel(),
                      _lib.stream_handle(dev))
         return gx, gw, gb, None, None, None, None
+
+
+def _gaps(*tensors) -> bool:
+    """Whether one of them (None: none) is not contiguous."""
+    for t in tensors:
+        if t is not None and not t.is_contiguous():
+            return True
+    return False
 
 
 def _packed(t):
@@ -519,7 +531,10 @@ def group_norm(x: torch.Tensor, num_groups: int, weight: Optional[torch.Tensor] 
     shape = x.shape
     if ptr is None:
         x = x.unsqueeze(1) if x.dim() == 2 else x.flatten(1, -2)
-    x, weight, bias = _unit_rows(x), _packed(weight), _packed(bias)
+    if C > 1 and x.stride(-1) != 1:
+        x = x.contiguous()
+    weight = weight.contiguous() if weight is not None else None
+    bias = bias.contiguous() if bias is not None else None
     args = (x, weight, bias, ptr, int(num_groups), float(eps), ACTIVATIONS[act])
     y = _GroupNorm.apply(*args) if _needs_grad(x, weight, bias) else _group_norm_fwd(*args, False)[0]
     return y if y.shape == shape else y.view(shape)
@@ -534,7 +549,8 @@ class ClassLogProbs(NamedTuple):
 
 
 def _class_log_probs_fwd(logits, target, top, ignore_index, keep=False):
-    """(logp, entropy, top_logp, top_class, statistics or None)."""
+    """(logp, entropy, top_logp, top_class, statistics or None, the leading arguments of the C
+    calls)."""
     dev = logits.device
     rows, classes = logits.shape
     f32 = dict(dtype=torch.float32, device=dev)
@@ -547,12 +563,13 @@ def _class_log_probs_fwd(logits, target, top, ignore_index, keep=False):
     stats = torch.empty((rows, 2), **f32) if keep else None
     behind = -(-nbytes // 16) * 16
     ws = _ws(nbytes if keep else behind + 8 * rows, dev) if nbytes or not keep else None
-    _lib.call_on(dev, "gfd_class_logp_fwd", logits.data_ptr(), _ROW_DTYPES[logits.dtype], rows,
-                 classes, logits.stride(0), _lib.ptr(target), ignore_index, top, _lib.ptr(logp),
-                 entropy.data_ptr(), top_logp.data_ptr(), top_class.data_ptr(),
-                 stats.data_ptr() if keep else ws.data_ptr() + behind, _lib.ptr(ws), nbytes,
+    shape = (_ROW_DTYPES[logits.dtype], rows, classes, logits.stride(0))
+    _lib.call_on(dev, "gfd_class_logp_fwd", logits.data_ptr(), *shape, _lib.ptr(target),
+                 ignore_index, top, _lib.ptr(logp), entropy.data_ptr(), top_logp.data_ptr(),
+                 top_class.data_ptr(), stats.data_ptr() if keep else ws.data_ptr() + behind,
+                 _lib.ptr(ws), nbytes,
                  _lib.stream_handle(dev))
-    return logp, entropy, top_logp, top_class, stats
+    return logp, entropy, top_logp, top_class, stats, shape
 
 
 class _ClassLogProbs(torch.autograd.Function):
@@ -561,10 +578,10 @@ class _ClassLogProbs(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx, logits, target, top, ignore_index):
-        logp, entropy, top_logp, top_class, stats = _class_log_probs_fwd(
+        logp, entropy, top_logp, top_class, stats, ctx.shape = _class_log_probs_fwd(
             logits, target, top, ignore_index, True)
         ctx.save_for_backward(logits, target, entropy, top_class, stats)
-        ctx.top, ctx.ignore_index = top, ignore_index
+        ctx.top, ctx.ignore_index, ctx.strides = top, ignore_index, logits.stride()
         ctx.mark_non_differentiable(top_class)
         ctx.set_materialize_grads(False)
         return logp, entropy, top_logp, top_class
@@ -572,17 +589,20 @@ class _ClassLogProbs(torch.autograd.Function):
     @staticmethod
     @once_differentiable
     def backward(ctx, g_logp, g_entropy, g_top, _):
-        # saved-tensor hooks may bring them back elsewhere and in other strides
         logits, target, entropy, top_class, stats = ctx.saved_tensors
-        logits = _unit_rows(logits)
-        target, entropy, top_class, stats = map(_packed, (target, entropy, top_class, stats))
+        shape = ctx.shape
+        if logits.stride() != ctx.strides or _gaps(target, entropy, top_class, stats):
+            # saved-tensor hooks brought them back in other strides
+            logits = _unit_rows(logits)
+            target, entropy, top_class, stats = map(_packed, (target, entropy, top_class, stats))
+            shape = shape[:3] + (logits.stride(0),)
         dev = logits.device
         g_logp, g_entropy, g_top = map(_packed, (g_logp, g_entropy, g_top))
         grad = torch.empty(logits.shape, dtype=logits.dtype, device=dev)
-        _lib.call_on(dev, "gfd_class_logp_bwd", logits.data_ptr(), _ROW_DTYPES[logits.dtype],
-                     *logits.shape, logits.stride(0), _lib.ptr(target), ctx.ignore_index, ctx.top,
-                     top_class.data_ptr(), stats.data_ptr(), entropy.data_ptr(), _lib.ptr(g_logp),
-                     _lib.ptr(g_entropy), _lib.ptr(g_top), grad.data_ptr(), _lib.stream_handle(dev))
+        _lib.call_on(dev, "gfd_class_logp_bwd", logits.data_ptr(), *shape, _lib.ptr(target),
+                     ctx.ignore_index, ctx.top, top_class.data_ptr(), stats.data_ptr(),
+                     entropy.data_ptr(), _lib.ptr(g_logp), _lib.ptr(g_entropy), _lib.ptr(g_top),
+                     grad.data_ptr(), _lib.stream_handle(dev))
         return grad, None, None, None
 
 

@@ -43,7 +43,6 @@ _grad, _dtype, _layout = attrgetter("grad"), attrgetter("dtype"), attrgetter("la
 _data_ptr, _numel, _device, _contiguous = (torch.Tensor.data_ptr, torch.Tensor.numel,
                                            torch.Tensor.get_device, torch.Tensor.is_contiguous)
 _NONE = type(None)
-_STATES = ("step", "exp_avg", "exp_avg_sq", "exp_avg_scale", "exp_avg_sq_scale")
 
 
 def _dense(p: torch.Tensor) -> bool:
@@ -161,6 +160,8 @@ class Adam(torch.optim.Optimizer):
             for k in ("exp_avg", "exp_avg_sq"):
                 f[k] = torch.zeros(total, dtype=torch.uint8, device=dev).view(torch.float8_e4m3fn)
                 f[k + "_scale"] = torch.zeros(total // STATE_BLOCK, dtype=torch.float32, device=dev)
+        f["plain"] = f["strides"].count(None) == len(params)
+        f["states"] = [t for k, t in f.items() if isinstance(t, torch.Tensor) and k != "ticket"]
         # gfd_adam_tensor of every parameter; the two pointers are filled in at each step
         f["table"] = np.array([(0, 0, p.numel(), at, i) for i, (p, at) in enumerate(zip(params, first))],
                               dtype=np.int64)
@@ -284,9 +285,8 @@ class Adam(torch.optim.Optimizer):
 
     @staticmethod
     def _raise_versions(f, params: list) -> None:
-        # the flat buffers share theirs with the views of them
-        states = [f[k] for k in _STATES if k in f] if f is not None else []
-        torch.autograd.graph.increment_version(params + states)
+        # (the flat buffers share theirs with the views of them)
+        torch.autograd.graph.increment_version(params + f["states"] if f is not None else params)
 
     def _step_group(self, group: dict, f: dict) -> None:
         params = group["params"]
@@ -301,7 +301,7 @@ class Adam(torch.optim.Optimizer):
                 list(map(_device, params)).count(index) == n == list(map(_device, grads)).count(index) and
                 list(map(_numel, params)) == numel == list(map(_numel, grads)) and
                 all(map(_contiguous, params)) and all(map(_contiguous, grads)) and
-                f["strides"].count(None) == n):
+                f["plain"]):
             table = f["table"]
             table[:, 0] = list(map(_data_ptr, params))
             table[:, 1] = list(map(_data_ptr, grads))
