@@ -1,6 +1,11 @@
 """Shared test helpers (weights from fixtures, oracle CSR, tolerances)."""
 import numpy as np
 import torch
+import torch.multiprocessing
+
+# tensors in a queue by the names of files: by descriptors, which the sender serves, a rank that has
+# ended before its result is read leaves nothing to read (every rank imports this module)
+torch.multiprocessing.set_sharing_strategy("file_system")
 
 # Parity bar from BASELINE.json north_star: outputs within 1e-4 (fp32) of the
 # PyG-dataflow CPU forward on identical weights.
