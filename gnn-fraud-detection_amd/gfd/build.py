@@ -88,11 +88,11 @@ def _object_id(src: str, flags) -> str:
     return h.hexdigest()
 
 
-def _compile(src: str, objdir: str, flags) -> str:
+def _compile(src: str, objdir: str, flags, force: bool = False) -> str:
     obj = os.path.join(objdir, os.path.basename(src)[:-4] + ".o")
     oid = _object_id(src, flags)
     stamp = obj + ".sha256"
-    if os.path.exists(obj) and os.path.exists(stamp) and open(stamp).read().strip() == oid:
+    if not force and os.path.exists(obj) and os.path.exists(stamp) and open(stamp).read().strip() == oid:
         return obj   # built from exactly these bytes
     cmd = [HIPCC, *flags, *SOURCE_FLAGS.get(os.path.basename(src), []), "-c", src, "-o", obj]
     r = subprocess.run(cmd, capture_output=True, text=True)
@@ -154,10 +154,10 @@ def _build_one(lib: str, objdir: str, flags, force: bool, verbose: bool) -> str:
     if not force and not stale:
         return lib
     os.makedirs(objdir, exist_ok=True)
-    srcs = sources()   # (each object rebuilt unless its content stamp matches)
+    srcs = sources()   # (each object rebuilt unless its content stamp matches, or with force)
     workers = min(len(srcs), max(1, min(8, os.cpu_count() or 1)))
     with cf.ThreadPoolExecutor(workers) as ex:
-        objs = list(ex.map(lambda s: _compile(s, objdir, flags), srcs))
+        objs = list(ex.map(lambda s: _compile(s, objdir, flags, force), srcs))
     objs.append(_id_object(objdir, flags))
     tmp = lib + ".tmp"
     cmd = [HIPCC, f"--offload-arch={ARCH}", "-shared", "-fPIC", "-o", tmp, *objs]
