@@ -84,7 +84,8 @@ __device__ double power(double b, uint32_t t) {
   return r;
 }
 
-// 32-bit hash: two multiplications between shifts
+// 32-bit hash: two multiplications between shifts, with constants of C. Wellons' published search
+// for the least bias between input and output bits
 __device__ __forceinline__ uint32_t mix32(uint32_t h) {
   h ^= h >> 16;
   h *= 0x7FEB352Du;
@@ -346,6 +347,7 @@ __global__ void __launch_bounds__(kThreads, BITS == 32 ? kWaves32 : kWaves8) k_a
           rmax = max(rmax, finite_bits(r[j]));
         }
       }
+      // (v_rcp_f32 is within 2^-23: two roundings, of an update whose moments are known to 2^-4)
 #pragma unroll
       for (int j = 0; j < kPer; ++j)
         p[j] = fmaf(p[j], keep, -rate * (m[j] * __builtin_amdgcn_rcpf(fmaf(r[j], unbias, a.eps))));
