@@ -19,8 +19,9 @@
 //     their lists' last entries.
 // Rows of up to kNarrow classes are read by teams of 1 to 32 lanes, longer ones
 // by a wave, long ones by a block; few long rows are split over blocks whose
-// partial results a second kernel joins.  2048 rows of 203769 bf16 logits: 153 us
-// without a list (5.4 TB/s), 225 us with the best 8; backward 322 us.
+// partial results a second kernel joins.  2048 rows of 203769 bf16 logits: 153 to
+// 161 us without a list (5.2 to 5.4 TB/s), 190 to 201 us with the best 8; backward
+// 305 to 322 us.
 #include "gfd_rowops.h"
 
 using namespace gfd;

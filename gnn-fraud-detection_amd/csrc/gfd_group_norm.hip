@@ -650,8 +650,8 @@ constexpr int kTileThreads = 256;
 // column sums of a tile: forward [slot][vecs] of x - c and (x - c)^2, backward [slot][channels] of
 // dz and dz xhat; ragged tiles have two slots, an unused one is 0.  (These kernels are kept small:
 // with indexed pieces, 64-bit divisions and more rows in flight the sums of 26 MB in 49 ragged
-// segments took 22 us, so 11.  Of its waves' cycles there 41 to 58 % wait for memory, 12 to 26 %
-// for an instruction, of whose fetches 1 % miss.)
+// segments took 22 us, so 11.  Of their waves' cycles there 37 to 59 % wait for memory, 12 to 26 %
+// for an instruction, of whose fetches up to 1 % miss.)
 template <typename T, int V, bool BWD, int ACT>
 __device__ __forceinline__ void do_sums(const Norm& n, int64_t t, double2* red) {
   constexpr int S = BWD ? V : 1;
