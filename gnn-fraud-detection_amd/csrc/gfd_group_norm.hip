@@ -128,9 +128,10 @@ __device__ __forceinline__ const T* row_in(const Norm& n, const void* base, int6
                : p + seg * n.seg_stride + (r - seg * n.length) * n.row_stride;
 }
 
-// what the sums of a segment (with rows, the first one ``start``) and the group whose first channel
-// is ch are taken about in fp64: its first element.  However far from 0 the group lies, the sum of squares is at most its
-// number of elements times the spread's, so that of 53 bits only as many go as that number has
+// what the sums of a segment (with rows, the first one ``start``) and the group whose first
+// channel is ch are taken about in fp64: its first element.  However far from 0 the group lies,
+// the sum of squares is at most its number of elements times the spread's, so that of 53 bits
+// only as many go as that number has
 template <typename T>
 __device__ __forceinline__ T base_of(const Norm& n, int64_t seg, int64_t start, int ch) {
   return static_cast<const T*>(n.x)[(n.ptr ? start * n.row_stride : seg * n.seg_stride) + ch];
@@ -301,8 +302,8 @@ __device__ __forceinline__ double2 sum_rows(double2 v, int cols, double2* red) {
   return v;
 }
 
-// A thread's sums of x and x^2 about c, in fp32 about its own first element k and, every few rows, into
-// fp64 (a conversion to fp64 takes four times an fp32 operation): what rounding does to the
+// A thread's sums of x and x^2 about c, in fp32 about its own first element k and, every few rows,
+// into fp64 (a conversion to fp64 takes four times an fp32 operation): what rounding does to the
 // deviations from k, however far k lies from 0, is not multiplied by it.  The squares of the k -
 // mean of all threads are at most the sum of squares itself, so neither does an odd k cost digits.
 struct Shifted {

@@ -50,6 +50,11 @@ def _dense(p: torch.Tensor) -> bool:
     return p.is_contiguous() or torch.empty_like(p, device="meta").stride() == p.stride()
 
 
+def _strides(p: torch.Tensor):
+    """Of a parameter; None: contiguous."""
+    return None if p.is_contiguous() else p.stride()
+
+
 def _refuse(options: dict) -> None:
     for name in ("amsgrad", "maximize", "differentiable"):
         if options.get(name):
@@ -149,8 +154,7 @@ class Adam(torch.optim.Optimizer):
             total += -(-p.numel() // STATE_BLOCK) * STATE_BLOCK
         total = max(total, STATE_BLOCK)          # of parameters without elements too there is a buffer
         f = {"first": first, "numel": [p.numel() for p in params], "bits": bits, "device": dev,
-             # the strides that the states have too; None: contiguous
-             "strides": [None if p.is_contiguous() else p.stride() for p in params],
+             "strides": [_strides(p) for p in params],      # the states have them too
              "step": torch.zeros(len(params), dtype=torch.int32, device=dev),
              "ticket": torch.zeros(1056, dtype=torch.int32, device=dev)}
         if f["bits"] == 32:
@@ -189,9 +193,9 @@ class Adam(torch.optim.Optimizer):
     def load_state_dict(self, state_dict: dict) -> None:
         """Of this class, or of torch.optim.Adam / AdamW (fp32 states).  One that is refused leaves
         the optimizer as it was.  States of the same ``state_bits`` are filled where they are, and
-        so is an lr that is a tensor: a captured ``step()`` goes on from what was loaded (but for the numbers
-        among the options, which it holds).  With other ``state_bits`` the states are made anew,
-        and a captured step has to be captured again."""
+        so is an lr that is a tensor: a captured ``step()`` goes on from what was loaded (but for
+        the numbers among the options, which it holds).  With other ``state_bits`` the states are
+        made anew, and a captured step has to be captured again."""
         groups = []
         for g, mine in zip(state_dict["param_groups"], self.param_groups):
             groups.append({**{k: mine[k] for k in ("state_bits", "seed", "decoupled_weight_decay")}, **g})
@@ -211,18 +215,19 @@ class Adam(torch.optim.Optimizer):
             to.copy_(t) if t is not None else to.zero_()
 
     def _load_group(self, gi: int, keys: list, states: dict, before: tuple, copies: list) -> None:
-        flat, state, old_groups = before
+        flat, _, old_groups = before
         group, old, f = self.param_groups[gi], old_groups[gi], flat.get(gi)
         self._check_group(group)
         known = any(k in states for k in keys)
         # one that cannot be gone on with (other bits, parameters added, moved or laid out anew) is
         # made anew
-        if (f is not None and f["bits"] == group["state_bits"] and len(f["first"]) == len(group["params"]) and
-                all(p.get_device() == f["device"].index and state[p]["exp_avg"].shape == p.shape and
-                    state[p]["exp_avg"].stride() == p.stride() for p in group["params"])):
+        if (f is not None and f["bits"] == group["state_bits"] and
+                f["numel"] == [p.numel() for p in group["params"]] and
+                f["strides"] == [_strides(p) for p in group["params"]] and
+                all(p.get_device() == f["device"].index for p in group["params"])):
             self._flat[gi] = f
-            for p in group["params"]:
-                self.state[p] = state[p]
+            for i, p in enumerate(group["params"]):
+                self.state[p] = self._views(f, i, p)
         elif known:
             self._group_state(gi)
         if gi in self._flat:
@@ -301,12 +306,11 @@ class Adam(torch.optim.Optimizer):
                 list(map(_device, params)).count(index) == n == list(map(_device, grads)).count(index) and
                 list(map(_numel, params)) == numel == list(map(_numel, grads)) and
                 all(map(_contiguous, params)) and all(map(_contiguous, grads)) and
-                f["plain"]):
+                f["plain"] and dtype in _CODES):
             table = f["table"]
             table[:, 0] = list(map(_data_ptr, params))
             table[:, 1] = list(map(_data_ptr, grads))
-            self._launch(group, f, dtype, table)
-            self._raise_versions(f, params)
+            self._launch(group, f, dtype, table, params)
             return
         self._step_mixed(group, f)
 
@@ -317,7 +321,6 @@ class Adam(torch.optim.Optimizer):
         index = dev.index
         tables: Dict[torch.dtype, Tuple[list, list, list]] = {}
         kept = []                       # copies of gradients, alive until the launch is queued
-        stepped = []
         dtype = params = grads = places = None
         for i, p in enumerate(group["params"]):
             g = p.grad
@@ -326,6 +329,8 @@ class Adam(torch.optim.Optimizer):
             if p.dtype is not dtype:
                 dtype = p.dtype
                 params, grads, places = tables.setdefault(dtype, ([], [], []))
+                if dtype not in _CODES:
+                    raise RuntimeError(f"gfd Adam: a parameter changed its type to {dtype}")
             if (g.dtype is not dtype or g.is_sparse or g.get_device() != index or
                     p.get_device() != index):
                 raise RuntimeError(f"gfd Adam: a gradient must be dense, {dtype} and on {dev} like its "
@@ -333,7 +338,7 @@ class Adam(torch.optim.Optimizer):
             n = numel[i]
             if p.numel() != n or g.numel() != n:
                 raise RuntimeError(f"gfd Adam: a parameter changed its size from {n} to {p.numel()}")
-            if (None if p.is_contiguous() else p.stride()) != f["strides"][i]:
+            if _strides(p) != f["strides"][i]:
                 raise RuntimeError("gfd Adam: a parameter changed its strides to "
                                    f"{p.stride()} after its states were made")
             if not (p.is_contiguous() and g.is_contiguous()) and g.stride() != p.stride():
@@ -342,22 +347,18 @@ class Adam(torch.optim.Optimizer):
             params.append(p.data_ptr())
             grads.append(g.data_ptr())
             places.append(i)
-            stepped.append(p)
         for dtype, (params, grads, places) in tables.items():
             table = f["table"][places]
             table[:, 0] = params
             table[:, 1] = grads
-            self._launch(group, f, dtype, table)
-        self._raise_versions(f, stepped)
+            self._launch(group, f, dtype, table, [group["params"][i] for i in places])
 
-    def _launch(self, group: dict, f: dict, dtype: torch.dtype, table: np.ndarray) -> None:
+    def _launch(self, group: dict, f: dict, dtype: torch.dtype, table: np.ndarray, params: list) -> None:
         dev, lr, lr_ptr = f["device"], group["lr"], None
         if isinstance(lr, torch.Tensor):
             if lr.device != dev:
                 raise RuntimeError(f"gfd Adam: lr is on {lr.device}, expected {dev}")
             lr, lr_ptr = 0.0, lr.data_ptr()
-        if dtype not in _CODES:
-            raise RuntimeError(f"gfd Adam: a parameter changed its type to {dtype}")
         b1, b2 = group["betas"]
         _check_apart(table, dtype.itemsize)
         _lib.call_on(dev, "gfd_adam_step", table.ctypes.data, len(table), _CODES[dtype], f["bits"],
@@ -366,6 +367,7 @@ class Adam(torch.optim.Optimizer):
                      f["step"].data_ptr(), float(lr), lr_ptr, float(b1), float(b2),
                      float(group["eps"]), float(group["weight_decay"]), 1 if self._decoupled else 0,
                      int(group["seed"]), f["ticket"].data_ptr(), _lib.stream_handle(dev))
+        self._raise_versions(f, params)
 
 
 def _check_apart(table: np.ndarray, itemsize: int) -> None:

@@ -744,3 +744,18 @@ def test_the_options_of_torch():
                 cls([{"params": [p], name: True}])
         with pytest.raises(TypeError):
             cls([p], decay=1.0)
+
+
+def test_a_load_after_the_states_were_dropped(monkeypatch):
+    """``opt.state`` cleared by hand, and a group of no parameters beside: the load fills the
+    buffers, and the views are there again."""
+    p = torch.zeros(300, requires_grad=True)
+    opt, _ = _on_the_host(monkeypatch, [p])
+    opt.flat_state()["exp_avg"].fill_(2.0)
+    saved = copy.deepcopy(opt.state_dict())
+    opt.flat_state()["exp_avg"].zero_()
+    opt.state.clear()
+    opt.load_state_dict(saved)
+    assert (opt.state[p]["exp_avg"] == 2.0).all()
+    opt.param_groups.append(dict(opt.param_groups[0], params=[]))
+    opt.mark_stepped()
